@@ -12,5 +12,5 @@ from .attention import (  # noqa: F401
     Attention, decode_noalloc, kv_append, merge_partials, merge_partials_list, qk_norm_rope_append, rms_norm,
 )
 from .kv_cache import StaticKVCache  # noqa: F401
-from .projection import MatMul3, MatMulAdd  # noqa: F401
+from .projection import MatMul3, MatMulAdd, MatMulAddW4, pack_int4  # noqa: F401
 from .rope import precompute_freqs_cis  # noqa: F401

@@ -34,6 +34,13 @@ class AttnDesc(C.Structure):
     ]
 
 
+class AttnScores(C.Structure):
+    _fields_ = [
+        ("softcap", C.c_float), ("slopes", C.c_void_p), ("row_begin", C.c_void_p),
+        ("row_begin_stride", C.c_size_t), ("prefix_lens", C.c_void_p),
+    ]
+
+
 class MatMul3Desc(C.Structure):
     _fields_ = [
         ("hidden", C.c_void_p), ("hidden_row_stride", C.c_size_t), ("wq_nt", C.c_void_p), ("wk_nt", C.c_void_p),
@@ -53,6 +60,15 @@ class MatMulAddDesc(C.Structure):
         ("residual_row_stride", C.c_size_t), ("output", C.c_void_p), ("output_row_stride", C.c_size_t),
         ("m_max", C.c_size_t), ("n_max", C.c_size_t), ("k_max", C.c_size_t), ("max_batch", C.c_size_t),
         ("device", C.c_int), ("stream", C.c_void_p), ("async_", C.c_int),
+    ]
+
+
+class MatMulAddW4Desc(C.Structure):
+    _fields_ = [
+        ("a", C.c_void_p), ("a_row_stride", C.c_size_t), ("w4", C.c_void_p), ("scales", C.c_void_p),
+        ("zeros", C.c_void_p), ("group", C.c_size_t), ("residual", C.c_void_p), ("residual_row_stride", C.c_size_t),
+        ("output", C.c_void_p), ("output_row_stride", C.c_size_t), ("m_max", C.c_size_t), ("n_max", C.c_size_t),
+        ("k_max", C.c_size_t), ("max_batch", C.c_size_t), ("device", C.c_int), ("stream", C.c_void_p), ("async_", C.c_int),
     ]
 
 
@@ -89,6 +105,8 @@ _SIGNATURES = {
     "ellm_step_graph_launch": (_I, [_VP, _VP]),
     "ellm_step_graph_nodes": (_I, [_VP, C.POINTER(_SZ)]),
     "ellm_step_graph_destroy": (_I, [_VP]),
+    "ellm_attn_set_scores": (_I, [_VP, C.POINTER(AttnScores)]),
+    "ellm_attn_set_shared_prefix": (_I, [_VP, _VP, _VP, _SZ, _SZ, _SZ]),
     "ellm_attn_set_option": (_I, [_VP, C.c_char_p, C.c_longlong]),
     "ellm_attn_set_profiling": (_I, [_VP, _I]),
     "ellm_attn_kernel_stats": (_I, [_VP, _I, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.POINTER(C.c_double)]),
@@ -100,6 +118,9 @@ _SIGNATURES = {
     "ellm_matmul_add_create": (_I, [C.POINTER(MatMulAddDesc), C.POINTER(_VP)]),
     "ellm_matmul_add_destroy": (_I, [_VP]),
     "ellm_matmul_add_run": (_I, [_VP, _SZ, _SZ, _SZ, _SZ, _SZ]),
+    "ellm_matmul_add_w4_create": (_I, [C.POINTER(MatMulAddW4Desc), C.POINTER(_VP)]),
+    "ellm_matmul_add_w4_destroy": (_I, [_VP]),
+    "ellm_matmul_add_w4_run": (_I, [_VP, _SZ, _SZ, _SZ, _SZ, _SZ]),
     "ellm_matmul_set_profiling": (_I, [_VP, _I, _I]),
     "ellm_matmul_kernel_stats": (_I, [_VP, _I, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.POINTER(C.c_double)]),
     "ellm_matmul_check": (_I, [_VP, _I]),

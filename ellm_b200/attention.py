@@ -21,6 +21,14 @@ def _ptr(x):
     return x.data_ptr()
 
 
+def _check_tensor(name, t, dtype, shape):
+    """A torch tensor handed over as a device array: its type, size and place (raw pointers pass)."""
+    if t is None or not hasattr(t, "data_ptr"):
+        return
+    if str(t.dtype) != "torch." + dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor of shape {list(shape)}")
+
+
 class Attention:
     def __init__(self):
         raise TypeError("use Attention.new(...)")
@@ -101,6 +109,61 @@ class Attention:
             if status:
                 L.check(status)
         return step
+
+    def set_scores(self, softcap=0.0, slopes=None, row_begin=None, prefix_lens=None):
+        """Capped, biased and interval-masked scores for the runs that follow (ellm_attn_set_scores).
+
+        softcap: s -> softcap * tanh(s / softcap) (0 = none).  slopes: float32 [q_heads], s -> s - slopes[h] *
+        |pos - key|.  row_begin: int32 [max_batch, >= max_seq], the first key the row at each position sees
+        (document start, window start, pos + 1 for a row that sees nothing).  prefix_lens: int32 [max_batch],
+        positions every row of the sequence sees.  Tensors are device buffers read by every run; without any
+        argument the operator goes back to plain attention."""
+        d = self.desc
+        _check_tensor("slopes", slopes, "float32", (d.q_heads,))
+        _check_tensor("prefix_lens", prefix_lens, "int32", (d.max_batch,))
+        stride = d.max_seq
+        if hasattr(row_begin, "data_ptr"):
+            if str(row_begin.dtype) != "torch.int32" or row_begin.dim() != 2 or row_begin.shape[0] < d.max_batch \
+                    or row_begin.shape[1] < d.max_seq or row_begin.stride(1) != 1:
+                raise ValueError(f"row_begin must be int32 [{d.max_batch}, >= {d.max_seq}] with contiguous rows")
+            if not row_begin.is_cuda:
+                raise ValueError("row_begin must be a CUDA tensor")
+            # (the stride of a one-row tensor says nothing)
+            stride = row_begin.stride(0) if row_begin.shape[0] > 1 else row_begin.shape[1]
+        s = L.AttnScores(float(softcap), _ptr(slopes), _ptr(row_begin), stride, _ptr(prefix_lens))
+        L.check(self._lib.ellm_attn_set_scores(self._h, C.byref(s)))
+        self._keep_scores = (slopes, row_begin, prefix_lens)
+
+    def set_shared_prefix(self, k, v, prefix_len=None, strides=None):
+        """A prefix shared by all sequences of the batch (ellm_attn_set_shared_prefix): k and v
+        [kv_heads, rows, head_size] bf16, of which the first prefix_len rows count (default: all).  The handle's
+        cache and positions then count what follows the prefix.  With raw pointers, strides = (kv head, position)
+        in elements.  k = None removes it."""
+        if k is None:
+            L.check(self._lib.ellm_attn_set_shared_prefix(self._h, None, None, 0, 0, 0))
+            self._keep_prefix = None
+            return
+        if hasattr(k, "data_ptr"):
+            for name, t in (("k", k), ("v", v)):
+                if str(t.dtype) != "torch.bfloat16" or not t.is_cuda or t.dim() != 3 or t.stride(2) != 1 \
+                        or t.shape[0] < self.desc.kv_heads or t.shape[2] != self.desc.head_size:
+                    raise ValueError(f"{name} must be a bf16 CUDA tensor [{self.desc.kv_heads}, rows, {self.desc.head_size}] "
+                                     "with contiguous rows")
+            if k.shape != v.shape or k.stride() != v.stride():
+                raise ValueError("k and v must have the same shape and strides")
+            if prefix_len is None:
+                prefix_len = k.shape[1]
+            if not 0 <= prefix_len <= k.shape[1]:
+                raise ValueError(f"prefix_len {prefix_len} outside [0, {k.shape[1]}]")
+            if strides is None:
+                # (strides over one head or one row say nothing)
+                ps = k.stride(1) if k.shape[1] > 1 else k.shape[2]
+                strides = (k.stride(0) if k.shape[0] > 1 else k.shape[1] * ps, ps)
+        if prefix_len is None or strides is None:
+            raise ValueError("raw pointers need prefix_len and strides")
+        L.check(self._lib.ellm_attn_set_shared_prefix(self._h, _ptr(k), _ptr(v), int(strides[0]), int(strides[1]),
+                                                      int(prefix_len)))
+        self._keep_prefix = (k, v)
 
     def set_option(self, name, value):
         L.check(self._lib.ellm_attn_set_option(self._h, name.encode(), int(value)))

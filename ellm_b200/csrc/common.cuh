@@ -251,9 +251,10 @@ __device__ __forceinline__ void qk_step(const uint32_t (&qf)[8][4], uint32_t k_b
 // Thread layout: of every S^T / O^T fragment a thread owns heads (lane%4)*2, +1 of the block and
 // keys (or dims) lane/4 and lane/4 + 8 - so the running maximum m and the sum l of a head live in
 // the 8 lanes that share lane%4; l holds this thread's keys only until the piece is finalised.
-template <int NB>
+// score(t, nb, h, key) turns the product of (block nb's head (lane%4)*2 + h, key) into log2 units.
+template <int NB, class Score>
 __device__ __forceinline__ void decode_stage_t(const uint32_t (&qb)[NB][8][2], uint32_t k_base, uint32_t v_base,
-                                               long long kfirst, long long len, float scale_log2, float (&m)[NB][2],
+                                               long long kfirst, long long len, const Score& score, float (&m)[NB][2],
                                                float (&l)[NB][2], float (&oT)[NB][8][4], int lane) {
     const int mat = lane >> 3, mrow = lane & 7;
     float s[NB][4];
@@ -276,8 +277,8 @@ __device__ __forceinline__ void decode_stage_t(const uint32_t (&qb)[NB][8][2], u
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float s_lo = in_lo ? s[nb][h] * scale_log2 : -INFINITY;
-            const float s_hi = in_hi ? s[nb][h + 2] * scale_log2 : -INFINITY;
+            const float s_lo = in_lo ? score(s[nb][h], nb, h, kfirst + (lane >> 2)) : -INFINITY;
+            const float s_hi = in_hi ? score(s[nb][h + 2], nb, h, kfirst + (lane >> 2) + 8) : -INFINITY;
             float mx = fmaxf(s_lo, s_hi);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));

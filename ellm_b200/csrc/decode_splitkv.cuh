@@ -30,6 +30,7 @@
 // to 8 heads, else 2).
 #pragma once
 #include "common.cuh"
+#include "score_mods.cuh"
 
 namespace ellm {
 
@@ -40,6 +41,7 @@ constexpr int kDecStages = 3;                     // cp.async ring depth per war
 constexpr int kDecWarpStageBytes = 16 * kRowBytes * 2;  // 16 K rows + 16 V rows = 8 KB
 constexpr int kDecMaxBatch = 1024;                // prefix table held in shared memory
 constexpr int kDecSmemBytes = kDecWarps * kDecStages * kDecWarpStageBytes + (2 * kDecMaxBatch + 1) * 4;
+constexpr int kDecModsSmemBytes = kDecSmemBytes + kDecMaxBatch * 4;   // one more table: each sequence's first key
 
 struct DecodeParams {
     const __nv_bfloat16* q;        // [max_batch, q_heads, 128] (chunk row 0)
@@ -69,6 +71,8 @@ struct DecodeParams {
     // Only what that kernel cannot have written is touched early: the positions, and cache rows
     // below each sequence's newest row; the queries and the stages that hold a newest row wait.
     int early = 0;
+    // kMods instantiations: capped / biased scores, keys from row_begin[b][position] on (key_begin is 0)
+    ScoreMods mods;
 };
 
 // CTA index owning tile t under assign_range(total, n, .)
@@ -83,9 +87,9 @@ __device__ __forceinline__ long long dec_seq_len_raw(const DecodeParams& p, int 
     return p.positions ? static_cast<long long>(p.positions[b]) + 1 : p.uniform_len;
 }
 
-// Tiles of a sequence of `len` keys (all of its segments have the same count).
-__device__ __forceinline__ int dec_tiles_of(const DecodeParams& p, long long len) {
-    const long long n = len - p.key_begin;
+// Tiles of a sequence of `len` keys from `begin` on (all of its segments have the same count).
+__device__ __forceinline__ int dec_tiles_of(long long begin, long long len) {
+    const long long n = len - begin;
     if (n <= 0) return 0;
     return static_cast<int>((n + kDecTileKeys - 1) / kDecTileKeys);
 }
@@ -95,11 +99,19 @@ __device__ __forceinline__ int dec_tiles_of(const DecodeParams& p, long long len
 // again: they may live in page-locked host memory).  All threads call.  The positions are fetched by as many threads as there are
 // sequences (one global-memory latency, not one per sequence); the running sum over the
 // per-sequence tile counts is then a short loop over shared memory.
-__device__ inline void dec_build_prefix(const DecodeParams& p, int* prefix, int* lens) {
+// kMods: the keys start at row_begin[b][position]; begs[b] receives that (where begs is given).
+template <bool kMods = false>
+__device__ inline void dec_build_prefix(const DecodeParams& p, int* prefix, int* lens, int* begs = nullptr) {
     for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
         const long long raw = dec_seq_len_raw(p, b);
         lens[b] = static_cast<int>(raw < 0 ? 0 : raw);
-        prefix[b + 1] = dec_tiles_of(p, raw < p.len_cap ? raw : p.len_cap);
+        long long begin = p.key_begin;
+        if constexpr (kMods) {
+            long long hi;
+            row_interval(p.mods, b, raw - 1, p.len_cap, begin, hi);
+            if (begs) begs[b] = static_cast<int>(begin);
+        }
+        prefix[b + 1] = dec_tiles_of(begin, raw < p.len_cap ? raw : p.len_cap);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -176,11 +188,28 @@ __device__ inline bool dec_aligned_range(const DecodeParams& p, const int* prefi
     return false;
 }
 
+struct PlainScore {
+    float scale_log2;
+    __device__ __forceinline__ float operator()(float t, int, int, long long) const { return t * scale_log2; }
+};
+// The capped / biased score of a decode step.  Streaming K/V is what bounds the step, so the tanh takes
+// its direct form (two special-function operations for each of a lane's 4 scores per 16 keys).
 template <int NB>
+struct ModScore {
+    const ScoreMods& mods;
+    float slope_log2[NB][2];
+    long long pos;
+    __device__ __forceinline__ float operator()(float t, int nb, int h, long long key) const {
+        return mod_score(mods, t, slope_log2[nb][h], static_cast<float>(static_cast<int>(pos - key)));
+    }
+};
+
+template <int NB, bool kMods = false>
 __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const DecodeParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     int* prefix = reinterpret_cast<int*>(smem + kDecWarps * kDecStages * kDecWarpStageBytes);   // [kDecMaxBatch + 1]
     int* lens = prefix + kDecMaxBatch + 1;                                                        // [kDecMaxBatch]
+    int* begs = kMods ? lens + kDecMaxBatch : nullptr;                                            // [kDecMaxBatch]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t warp_smem = smem_u32(smem) + warp * kDecStages * kDecWarpStageBytes;
     ChainTrace ct(2);
@@ -196,7 +225,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         ct.waited();
     }
-    dec_build_prefix(p, prefix, lens);
+    dec_build_prefix<kMods>(p, prefix, lens, begs);
     const long long segs_per_seq = static_cast<long long>(p.kv_heads) * p.gtiles;
     const long long total = static_cast<long long>(prefix[p.batch]) * segs_per_seq;
     long long t_begin = 0, t_end = 0;
@@ -224,7 +253,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
         const long long len_raw = lens[b];
         const long long len = len_raw < p.len_cap ? len_raw : p.len_cap;
         const int rows_valid = min(16, p.group - gt * 16);
-        const long long key0 = p.key_begin + static_cast<long long>(tile0) * kDecTileKeys + warp * 16;
+        const long long key0 = (kMods ? static_cast<long long>(begs[b]) : p.key_begin) + static_cast<long long>(tile0) * kDecTileKeys + warp * 16;
         const __nv_bfloat16* kbase = p.k_cache + b * p.s0 + kvh * p.s1;
         const __nv_bfloat16* vbase = p.v_cache + b * p.s0 + kvh * p.s1;
         // fused append: position of the new token's row and where its K/V come from
@@ -321,6 +350,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
             }
         }
 
+        float slopes[NB][2] = {};   // kMods: of this lane's heads, times log2(e)
+        if constexpr (kMods) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int head = nb * 8 + (lane & 3) * 2 + h;
+                    if (p.mods.slopes && head < rows_valid) slopes[nb][h] = p.mods.slopes[kvh * p.group + gt * 16 + head] * kLog2e;
+                }
+        }
         float hm[NB][2], hl[NB][2], oT[NB][8][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -338,7 +377,16 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
             const long long kfirst = key0 + static_cast<long long>(it) * kDecTileKeys;
             if (kfirst < len) {  // warp-uniform: this warp's 16 keys are not all past the end
                 const uint32_t sK = warp_smem + (it % kDecStages) * kDecWarpStageBytes;
-                decode_stage_t<NB>(qb, sK, sK + 16 * kRowBytes, kfirst, len, p.scale_log2, hm, hl, oT, lane);
+                if constexpr (kMods) {
+                    ModScore<NB> score{p.mods, {}, len_raw - 1};
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) score.slope_log2[nb][h] = slopes[nb][h];
+                    decode_stage_t<NB>(qb, sK, sK + 16 * kRowBytes, kfirst, len, score, hm, hl, oT, lane);
+                } else {
+                    decode_stage_t<NB>(qb, sK, sK + 16 * kRowBytes, kfirst, len, PlainScore{p.scale_log2}, hm, hl, oT, lane);
+                }
             }
             __syncwarp();  // all lanes done with this stage before it is refilled
         }

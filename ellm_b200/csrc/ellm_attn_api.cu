@@ -23,6 +23,7 @@
 #include "prefill_tcgen05.cuh"
 #include "qk_norm_rope_append.cuh"
 #include "rms_norm.cuh"
+#include "score_mods.cuh"
 
 namespace ellm {
 
@@ -158,6 +159,8 @@ struct ellm_attn {
                                        // are the prefill kernel's work-list counters
     int* status_host = nullptr;        // pinned mirror
     ellm::Tcgen05Plan tc;              // tensor maps etc. of the tcgen05 prefill kernel
+    ellm::ScoreMods mods;              // ellm_attn_set_scores / ellm_attn_set_shared_prefix
+    bool scores_on = false, prefix_on = false;
     std::mutex mu;
     uint64_t launches[ELLM_KERNEL_COUNT] = {};
     uint64_t timed[ELLM_KERNEL_COUNT] = {};
@@ -262,7 +265,7 @@ int launch_append(ellm_attn* h, cudaStream_t stream, void* k_cache, void* v_cach
 // the light shape (2 warps per row, tables in dynamic shared memory), few rows with many pieces the
 // wide one.  A row's pieces are at most the decode grid's CTAs.
 cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blocks, float* out_f32, void* out_bf16,
-                         float* lse_out, cudaStream_t stream, bool dependent) {
+                         float* lse_out, cudaStream_t stream, bool dependent, bool mods = false) {
     const int pieces_cap = std::min(p.num_ctas, ellm::kMergeMaxPieces);
     const size_t smem = ellm::merge_smem_bytes(static_cast<int>(batch), pieces_cap);
     const bool light = blocks >= 128;
@@ -277,6 +280,9 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 1 : 0;
     __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out_bf16);
+    if (mods)   // (the pieces of a row follow from its own first key)
+        return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, true>, p, ob, lse_out, pieces_cap)
+                     : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, true>, p, ob, lse_out, pieces_cap);
     if (out_f32)
         return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 2, 4>, p, out_f32, lse_out, pieces_cap)
                      : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 8, 10>, p, out_f32, lse_out, pieces_cap);
@@ -313,6 +319,7 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
     p.gtiles = h->gtiles;
     p.scale_log2 = h->d.scale * ellm::kLog2e;
     p.num_ctas = h->dec_ctas;
+    p.mods = h->mods;
     if (append) {   // the new token's K/V rows ride along with the decode kernel
         p.k_new = static_cast<const __nv_bfloat16*>(h->d.k_new);
         p.v_new = static_cast<const __nv_bfloat16*>(h->d.v_new);
@@ -321,7 +328,12 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
     }
     {
         LaunchScope ls(h, ELLM_KERNEL_DECODE_SPLITKV);
-        if (h->group <= 8)   // blocks of 8 query heads per segment: one for groups of up to 8 heads, else two
+        if (h->scores_on) {
+            if (h->group <= 8)
+                launch_dependent(ellm::decode_splitkv_kernel<1, true>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
+            else
+                launch_dependent(ellm::decode_splitkv_kernel<2, true>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
+        } else if (h->group <= 8)   // blocks of 8 query heads per segment: one for groups of up to 8 heads, else two
             launch_dependent(ellm::decode_splitkv_kernel<1>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
         else
             launch_dependent(ellm::decode_splitkv_kernel<2>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
@@ -333,7 +345,7 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
         // its first instruction waits for the decode grid's memory to be visible
         LaunchScope ls(h, ELLM_KERNEL_MERGE);
         const cudaError_t e = launch_merge(p, batch, blocks, out_f32, out_f32 ? nullptr : (out_override ? out_override : h->d.out),
-                                           lse_out, h->stream, true);
+                                           lse_out, h->stream, true, h->scores_on);
         if (e != cudaSuccess) return fail(ELLM_ERR_CUDA, "merge launch failed: %s", cudaGetErrorString(e));
     }
     ELLM_CUDA(cudaGetLastError());
@@ -342,12 +354,12 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
 
 int launch_prefill_warp_mma(ellm_attn* h, const int32_t* positions, size_t position_index,
                             size_t interval, size_t batch, long long key_begin, long long key_end,
-                            float* out_f32, float* lse_out) {
+                            float* out_f32, float* lse_out, void* out_override = nullptr) {
     ellm::PrefillParams p;
     p.q = static_cast<const __nv_bfloat16*>(h->d.q);
     p.k_cache = static_cast<const __nv_bfloat16*>(h->d.k_cache);
     p.v_cache = static_cast<const __nv_bfloat16*>(h->d.v_cache);
-    p.out = out_f32 ? static_cast<void*>(out_f32) : h->d.out;
+    p.out = out_f32 ? static_cast<void*>(out_f32) : (out_override ? out_override : h->d.out);
     p.lse = lse_out;
     p.positions = positions;
     p.position_index = static_cast<long long>(position_index);
@@ -364,10 +376,13 @@ int launch_prefill_warp_mma(ellm_attn* h, const int32_t* positions, size_t posit
     p.scale_log2 = h->d.scale * ellm::kLog2e;
     if (batch > 65535 || h->d.kv_heads > 65535)
         return fail(ELLM_ERR_UNSUPPORTED, "batch / kv_heads exceed the grid limit 65535");
+    p.mods = h->mods;
     dim3 grid(p.row_tiles, p.kv_heads, p.batch);
     {
         LaunchScope ls(h, ELLM_KERNEL_PREFILL_WARP_MMA);
-        if (out_f32)
+        if (h->scores_on || h->prefix_on)
+            ellm::prefill_warp_mma_kernel<__nv_bfloat16, true><<<grid, ellm::kPfThreads, ellm::kPfSmemBytes, h->stream>>>(p);
+        else if (out_f32)
             ellm::prefill_warp_mma_kernel<float><<<grid, ellm::kPfThreads, ellm::kPfSmemBytes, h->stream>>>(p);
         else
             ellm::prefill_warp_mma_kernel<__nv_bfloat16><<<grid, ellm::kPfThreads, ellm::kPfSmemBytes, h->stream>>>(p);
@@ -433,27 +448,35 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
     const bool no_sync = enqueue_only < 0 ? h->d.async != 0 : enqueue_only != 0;
     int rc;
     const bool do_append = append && h->d.k_new;
+    const bool ext = h->scores_on || h->prefix_on;
+    if (ext && out_f32)
+        return fail(ELLM_ERR_UNSUPPORTED, "a key window cannot be combined with modified scores or a shared prefix");
     // which kernel takes a chunk of more than one row
     bool use_tc = false;
     if (interval > 1) {
         if (h->d.prefill_kernel == ELLM_PREFILL_TCGEN05) use_tc = true;
         else if (h->d.prefill_kernel == ELLM_PREFILL_AUTO) use_tc = ellm::tcgen05_prefers(h->tc, interval, h->group);
+        if (ext) use_tc = false;
     }
     // the chunk's K/V rows go into the cache inside the attention kernel where that is possible (a decode
     // step always does; the tensor-memory prefill kernel when the chunk starts on a key-tile boundary),
     // else by the append kernel first
     const bool fused = use_tc && do_append && !out_f32 &&
                        ellm::tcgen05_can_fuse_append(h->tc, h->d, positions, position_index, batch, key_begin, key_end);
-    if (do_append && interval > 1 && !fused) {
+    // (a decode step whose rows may see nothing would not visit the newest row: appended up front as well)
+    const bool decode_appends = !h->prefix_on && !h->mods.row_begin;
+    if (do_append && (interval > 1 || !decode_appends) && !fused) {
         rc = launch_append(h, h->stream, h->d.k_cache, h->d.v_cache, h->d.k_new, h->d.v_new, h->d.kv_strides,
                            h->d.max_batch, h->d.kv_heads, h->d.max_seq, position_index, positions, interval, batch);
         if (rc) return rc;
     }
-    if (interval == 1) {
+    if (interval == 1 && h->prefix_on) {
+        rc = launch_prefill_warp_mma(h, positions, position_index, interval, batch, key_begin, key_end, nullptr, lse_out, decode_out_override);
+    } else if (interval == 1) {
         // early streaming only where the caller vouched for it, and never for a step whose inputs the
         // library itself stages right before (the host-buffer entry point passes a stream override)
-        rc = launch_decode(h, positions, position_index, batch, key_begin, key_end, out_f32, lse_out, do_append,
-                           decode_out_override, h->decode_early != 0 && stream_override == nullptr);
+        rc = launch_decode(h, positions, position_index, batch, key_begin, key_end, out_f32, lse_out, do_append && decode_appends,
+                           decode_out_override, h->decode_early != 0 && stream_override == nullptr && !ext);
     } else {
         if (use_tc) {
             if (!h->tc.ready)
@@ -535,6 +558,9 @@ int ellm_attn_create(const ellm_attn_desc* desc, ellm_attn** out) {
     if (cudaMemset(h->status_dev, 0, 4 * sizeof(int)) != cudaSuccess) return cleanup(fail(ELLM_ERR_CUDA, "memset failed"));
     if (cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<__nv_bfloat16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess)
         return cleanup(fail(ELLM_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(cudaGetLastError())));
@@ -1116,6 +1142,81 @@ int ellm_step_graph_destroy(ellm_step_graph* g) {
     DeviceGuard guard(g->device);
     if (g->exec) cudaGraphExecDestroy(g->exec);
     delete g;
+    return ELLM_OK;
+}
+
+// The captured host-buffer step holds the scores and the prefix it was captured with: built anew after a change.
+static void drop_host_step(ellm_attn* h) {
+    DeviceGuard guard(h->d.device);
+    if (h->graph_exec) cudaGraphExecDestroy(h->graph_exec);
+    h->graph_exec = nullptr;
+    h->graph_key = ellm_attn::HostStepKey();
+    h->graph_key_rejected = false;
+}
+
+int ellm_attn_set_scores(ellm_attn* h, const ellm_attn_scores* s) {
+    if (!h) return fail(ELLM_ERR_INVALID_ARG, "handle is NULL");
+    std::lock_guard<std::mutex> lock(h->mu);
+    const bool on = s && (s->softcap != 0.0f || s->slopes || s->row_begin || s->prefix_lens);
+    ellm::ScoreMods m;
+    if (on) {
+        if (h->prefix_on) return fail(ELLM_ERR_UNSUPPORTED, "modified scores cannot be combined with a shared prefix");
+        if (!(s->softcap >= 0.0f) || !std::isfinite(s->softcap)) return fail(ELLM_ERR_INVALID_ARG, "softcap must be finite and >= 0");
+        if (((reinterpret_cast<uintptr_t>(s->slopes) | reinterpret_cast<uintptr_t>(s->row_begin) |
+              reinterpret_cast<uintptr_t>(s->prefix_lens)) & 3u) != 0)
+            return fail(ELLM_ERR_INVALID_ARG, "slopes, row_begin and prefix_lens must be 4-byte aligned");
+        if (s->row_begin && s->row_begin_stride < h->d.max_seq)
+            return fail(ELLM_ERR_INVALID_ARG, "row_begin_stride %zu is below max_seq %zu", s->row_begin_stride, h->d.max_seq);
+        m.scale_log2 = h->d.scale * ellm::kLog2e;
+        if (s->softcap > 0.0f) {
+            m.cap_in = h->d.scale / s->softcap;
+            m.cap_log2 = s->softcap * ellm::kLog2e;
+            if (!(m.cap_in < INFINITY) || !(m.cap_log2 < INFINITY) || m.cap_in == 0.0f)
+                return fail(ELLM_ERR_INVALID_ARG, "softcap %g is out of range for scale %g", s->softcap, h->d.scale);
+        }
+        m.slopes = s->slopes;
+        m.row_begin = s->row_begin;
+        m.rb_stride = static_cast<long long>(s->row_begin_stride);
+        m.prefix_lens = s->prefix_lens;
+        m.max_seq = static_cast<long long>(h->d.max_seq);
+    } else if (h->prefix_on) {
+        return ELLM_OK;   // nothing to take back
+    }
+    h->mods = m;
+    h->scores_on = on;
+    drop_host_step(h);
+    return ELLM_OK;
+}
+
+int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size_t kv_head_stride, size_t position_stride,
+                                size_t prefix_len) {
+    if (!h) return fail(ELLM_ERR_INVALID_ARG, "handle is NULL");
+    std::lock_guard<std::mutex> lock(h->mu);
+    if ((k == nullptr) != (v == nullptr)) return fail(ELLM_ERR_INVALID_ARG, "k and v must be both set or both NULL");
+    const bool on = k && prefix_len > 0;
+    if (!on) {
+        if (!h->prefix_on) return ELLM_OK;
+        h->mods = ellm::ScoreMods();
+        h->prefix_on = false;
+        drop_host_step(h);
+        return ELLM_OK;
+    }
+    if (h->scores_on) return fail(ELLM_ERR_UNSUPPORTED, "a shared prefix cannot be combined with modified scores");
+    if (!aligned16(k) || !aligned16(v)) return fail(ELLM_ERR_INVALID_ARG, "k and v must be 16-byte aligned");
+    if (kv_head_stride == 0 || kv_head_stride % 8 != 0 || position_stride == 0 || position_stride % 8 != 0)
+        return fail(ELLM_ERR_INVALID_ARG, "kv_head_stride and position_stride must be non-zero multiples of 8 elements");
+    if (prefix_len > 0x7fffff00ull) return fail(ELLM_ERR_UNSUPPORTED, "prefix_len %zu too large", prefix_len);
+    ellm::ScoreMods m;
+    m.scale_log2 = h->d.scale * ellm::kLog2e;
+    m.max_seq = static_cast<long long>(h->d.max_seq);
+    m.pk = static_cast<const __nv_bfloat16*>(k);
+    m.pv = static_cast<const __nv_bfloat16*>(v);
+    m.ps1 = static_cast<long long>(kv_head_stride);
+    m.ps2 = static_cast<long long>(position_stride);
+    m.plen = static_cast<long long>(prefix_len);
+    h->mods = m;
+    h->prefix_on = true;
+    drop_host_step(h);
     return ELLM_OK;
 }
 

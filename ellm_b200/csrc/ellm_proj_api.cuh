@@ -4,11 +4,14 @@
 #include "../../include/ellm_proj.h"
 #include "proj_tcgen05.cuh"
 #include "proj_skinny.cuh"
+#include "proj_w4.cuh"
 
 struct ProjHandle {
-    int which = 0;                 // 0 = MatMul3, 1 = MatMulAdd
+    int which = 0;                 // 0 = MatMul3, 1 = MatMulAdd, 2 = MatMulAddW4
     ellm_matmul3_desc d3{};
     ellm_matmul_add_desc da{};
+    ellm_matmul_add_w4_desc dw{};
+    __nv_bfloat16* w4_scratch = nullptr;    // MatMulAddW4, more than 16 rows: the weights as bf16, written by every such run
     int device = 0;
     cudaStream_t stream = nullptr;
     bool async = false;
@@ -37,6 +40,7 @@ struct ProjHandle {
 };
 struct ellm_matmul3 : ProjHandle {};
 struct ellm_matmul_add : ProjHandle {};
+struct ellm_matmul_add_w4 : ProjHandle {};
 
 namespace {
 
@@ -73,6 +77,7 @@ void proj_common_destroy(ProjHandle* h) {
     }
     cudaFree(h->status_dev);
     cudaFree(h->qkv_scratch);
+    cudaFree(h->w4_scratch);
     if (h->status_host) cudaFreeHost(h->status_host);
 }
 
@@ -497,6 +502,147 @@ int ellm_matmul_add_run(ellm_matmul_add* h, size_t position_index, size_t positi
     p.ldr = static_cast<long long>(d.residual_row_stride ? d.residual_row_stride : d.n_max);
     p.n_cols = static_cast<int>(d.n_max);
     const size_t lda = d.a_row_stride ? d.a_row_stride : d.k_max;
+    return proj_launch(h, d.a, lda, d.k_max, rows, p);
+}
+
+}  // extern "C"
+
+namespace {
+
+typedef void (*W4Kernel)(const ellm::W4Params);
+template <int CB, int NB>
+W4Kernel w4_kernel_of(size_t group) {
+    return group == 128 ? ellm::proj_w4_kernel<CB, NB, 4> : group == 64 ? ellm::proj_w4_kernel<CB, NB, 2> : ellm::proj_w4_kernel<CB, NB, 1>;
+}
+// Column blocks per pass: as many as a CTA has (up to 4), so that a row fragment is fetched once for them.
+W4Kernel w4_kernel(int cb, int nb, size_t group) {
+    if (cb == 1) return nb == 1 ? w4_kernel_of<1, 1>(group) : w4_kernel_of<1, 2>(group);
+    if (cb == 2) return nb == 1 ? w4_kernel_of<2, 1>(group) : w4_kernel_of<2, 2>(group);
+    return nb == 1 ? w4_kernel_of<4, 1>(group) : w4_kernel_of<4, 2>(group);
+}
+int w4_column_blocks(size_t n, int sm_count) {
+    const size_t per_cta = ((n + 15) / 16 + sm_count - 1) / sm_count;
+    return per_cta >= 3 ? 4 : static_cast<int>(per_cta);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ellm_matmul_add_w4_create(const ellm_matmul_add_w4_desc* d, ellm_matmul_add_w4** out) {
+    if (!d || !out) return fail(ELLM_ERR_INVALID_ARG, "desc and out must be non-NULL");
+    *out = nullptr;
+    if (!d->a || !d->w4 || !d->scales || !d->output) return fail(ELLM_ERR_INVALID_ARG, "a, w4, scales and output must be non-NULL");
+    if (d->group != 32 && d->group != 64 && d->group != 128) return fail(ELLM_ERR_UNSUPPORTED, "group %zu: only 32, 64 or 128", d->group);
+    if (d->k_max == 0 || d->k_max % 128 != 0) return fail(ELLM_ERR_UNSUPPORTED, "k_max %zu must be a non-zero multiple of 128", d->k_max);
+    if (d->n_max == 0 || d->n_max % 8 != 0) return fail(ELLM_ERR_UNSUPPORTED, "n_max %zu must be a non-zero multiple of 8", d->n_max);
+    if (d->max_batch == 0 || d->m_max == 0 || d->m_max % d->max_batch != 0)
+        return fail(ELLM_ERR_INVALID_ARG, "m_max %zu must be a non-zero multiple of max_batch %zu", d->m_max, d->max_batch);
+    if (d->m_max > 0x7fffff00ull || d->n_max > 0x7fffff00ull || d->k_max > 0x7fffff00ull) return fail(ELLM_ERR_UNSUPPORTED, "matrix too large");
+    const size_t lda = d->a_row_stride ? d->a_row_stride : d->k_max;
+    const size_t ldr = d->residual_row_stride ? d->residual_row_stride : d->n_max;
+    const size_t ldc = d->output_row_stride ? d->output_row_stride : d->n_max;
+    if (!proj_stride_ok(lda, d->k_max) || !proj_stride_ok(ldr, d->n_max) || !proj_stride_ok(ldc, d->n_max))
+        return fail(ELLM_ERR_INVALID_ARG, "row strides must be multiples of 8 elements and cover a row");
+    if (!aligned16(d->a) || !aligned16(d->w4) || !aligned16(d->scales) || !aligned16(d->zeros) || !aligned16(d->residual) || !aligned16(d->output))
+        return fail(ELLM_ERR_INVALID_ARG, "buffers must be 16-byte aligned");
+    DeviceGuard guard(d->device);
+    if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", d->device);
+    ellm_matmul_add_w4* h = new (std::nothrow) ellm_matmul_add_w4();
+    if (!h) return fail(ELLM_ERR_NO_MEMORY, "out of host memory");
+    h->which = 2;
+    h->dw = *d;
+    int st = proj_common_create(h, d->device, d->stream, d->async);
+    if (st == ELLM_OK) {
+        const int cb = w4_column_blocks(d->n_max, h->plan.sm_count);
+        for (int nb = 1; nb <= 2 && st == ELLM_OK; ++nb)
+            if (cudaFuncSetAttribute(w4_kernel(cb, nb, d->group), cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::w4_smem_bytes(cb, nb)) != cudaSuccess)
+                st = fail(ELLM_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(cudaGetLastError()));
+    }
+    if (st == ELLM_OK && d->m_max > static_cast<size_t>(ellm::kW4MaxRows)) {
+        if (cudaMalloc(&h->w4_scratch, d->n_max * d->k_max * 2) != cudaSuccess) {
+            cudaGetLastError();
+            st = fail(ELLM_ERR_NO_MEMORY, "workspace allocation failed (%zu bytes)", d->n_max * d->k_max * 2);
+        } else if (!ellm::proj_encode_2d(h->plan, &h->map_w[0], h->w4_scratch, d->n_max, d->k_max, d->k_max, ellm::kPjBN) ||
+                   !ellm::proj_encode_2d(h->plan, &h->map_wp[0], h->w4_scratch, d->n_max, d->k_max, d->k_max, ellm::kPjBN / 2)) {
+            st = fail(ELLM_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled(weight) failed");
+        } else {
+            h->map_w[1] = h->map_w[2] = h->map_w[0];
+            h->map_wp[1] = h->map_wp[2] = h->map_wp[0];
+        }
+    }
+    if (st != ELLM_OK) {
+        proj_common_destroy(h);
+        delete h;
+        return st;
+    }
+    *out = h;
+    return ELLM_OK;
+}
+
+int ellm_matmul_add_w4_destroy(ellm_matmul_add_w4* h) {
+    if (!h) return ELLM_OK;
+    proj_common_destroy(h);
+    delete h;
+    return ELLM_OK;
+}
+
+int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t position_interval, size_t batch_size,
+                           size_t cpu_num, size_t thread_id) {
+    (void)position_index;
+    (void)cpu_num;
+    if (!h) return fail(ELLM_ERR_INVALID_ARG, "handle is NULL");
+    if (thread_id != 0) return ELLM_OK;
+    const ellm_matmul_add_w4_desc& d = h->dw;
+    if (batch_size > d.max_batch) return fail(ELLM_ERR_INVALID_ARG, "batch_size %zu > max_batch %zu", batch_size, d.max_batch);
+    if (position_interval > d.m_max / d.max_batch)
+        return fail(ELLM_ERR_INVALID_ARG, "position_interval %zu x max_batch %zu exceeds m_max %zu", position_interval, d.max_batch, d.m_max);
+    if (position_interval == 0 || batch_size == 0) return ELLM_OK;
+    std::lock_guard<std::mutex> lock(h->mu);
+    DeviceGuard guard(h->device);
+    if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", h->device);
+    const size_t rows = position_interval * d.max_batch;
+    const size_t lda = d.a_row_stride ? d.a_row_stride : d.k_max;
+    const long long ldc = static_cast<long long>(d.output_row_stride ? d.output_row_stride : d.n_max);
+    const long long ldr = static_cast<long long>(d.residual_row_stride ? d.residual_row_stride : d.n_max);
+    if (rows <= static_cast<size_t>(ellm::kW4MaxRows)) {
+        ellm::W4Params p{};
+        p.a = static_cast<const __nv_bfloat16*>(d.a);
+        p.lda = static_cast<long long>(lda);
+        p.w = static_cast<const uint8_t*>(d.w4);
+        p.scales = static_cast<const __nv_bfloat16*>(d.scales);
+        p.zeros = static_cast<const uint8_t*>(d.zeros);
+        p.residual = static_cast<const __nv_bfloat16*>(d.residual);
+        p.ldr = ldr;
+        p.c = static_cast<__nv_bfloat16*>(d.output);
+        p.ldc = ldc;
+        p.m_rows = static_cast<int>(rows);
+        p.batch = static_cast<int>(batch_size);
+        p.max_batch = static_cast<int>(d.max_batch);
+        p.n_cols = static_cast<int>(d.n_max);
+        p.k = static_cast<int>(d.k_max);
+        const int cb = w4_column_blocks(d.n_max, h->plan.sm_count), nb = rows > 8 ? 2 : 1;
+        const unsigned grid = static_cast<unsigned>(std::min<size_t>((d.n_max + 15) / 16, static_cast<size_t>(h->plan.sm_count)));
+        ELLM_CUDA(launch_dependent(w4_kernel(cb, nb, d.group), grid, ellm::kW4Threads, static_cast<size_t>(ellm::w4_smem_bytes(cb, nb)), h->stream, p));
+        ++h->skinny_launches;
+        return proj_finish(h);
+    }
+    const long long words = static_cast<long long>(d.n_max) * static_cast<long long>(d.k_max / 8);
+    const unsigned blocks = static_cast<unsigned>(std::min<long long>((words + 255) / 256, 8ll * h->plan.sm_count));
+    ELLM_CUDA(launch_dependent(ellm::w4_unpack_kernel, blocks, 256, 0, h->stream, static_cast<const uint32_t*>(d.w4),
+                               static_cast<const __nv_bfloat16*>(d.scales), static_cast<const uint8_t*>(d.zeros),
+                               reinterpret_cast<uint4*>(h->w4_scratch), words, static_cast<int>(d.k_max / 8), static_cast<int>(d.group / 8)));
+    ++h->skinny_launches;
+    ellm::ProjParams p{};
+    p.mode = ellm::kPjPlain;
+    p.tiles_n = static_cast<int>((d.n_max + ellm::kPjBN - 1) / ellm::kPjBN);
+    p.batch = static_cast<int>(batch_size);
+    p.max_batch = static_cast<int>(d.max_batch);
+    p.c = static_cast<__nv_bfloat16*>(d.output);
+    p.residual = static_cast<const __nv_bfloat16*>(d.residual);
+    p.ldc = ldc;
+    p.ldr = ldr;
+    p.n_cols = static_cast<int>(d.n_max);
     return proj_launch(h, d.a, lda, d.k_max, rows, p);
 }
 

@@ -49,7 +49,7 @@ __host__ __device__ inline size_t merge_smem_bytes(int batch, int pieces_cap) {
     return (static_cast<size_t>(2 * batch + 1) + static_cast<size_t>(pieces_cap)) * 4;
 }
 
-template <typename OutT, int kWarps, int kAhead>
+template <typename OutT, int kWarps, int kAhead, bool kMods = false>
 // (both shapes are held to 64 registers: they have to fit beside two decode CTAs of ~184 registers x 128 threads -
 // one wide CTA, or the light shape's three or four per SM - or they cannot move in, and release their own
 // dependents, before the decode grid has drained)
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
     // Where this row's pieces are follows from the positions alone, which are older than the decode
     // grid (it lets this grid start only after its own wait): the tile table is rebuilt here, before
     // the wait for the decode grid's results, instead of being read from it afterwards.
-    dec_build_prefix(p, s_prefix, s_lens);
+    dec_build_prefix<kMods>(p, s_prefix, s_lens);
     const long long row = blockIdx.x;
     const int b = static_cast<int>(row / p.q_heads), qh = static_cast<int>(row % p.q_heads);
     const int kvh = qh / p.group, g = qh % p.group, gt = g / 16, r = g % 16;

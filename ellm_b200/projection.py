@@ -11,7 +11,7 @@ torch CUDA tensors used as device buffers; raw integer device pointers work too.
 import ctypes as C
 
 from . import _lib as L
-from .attention import _ptr
+from .attention import _check_tensor, _ptr
 
 
 class _Projection:
@@ -126,6 +126,48 @@ class MatMulAdd(_Projection):
     def run(self, position_index, position_interval, batch_size, cpu_num=1, thread_id=0):
         L.check(self._lib.ellm_matmul_add_run(self._h, position_index, position_interval, batch_size, cpu_num,
                                               thread_id))
+
+
+class MatMulAddW4(_Projection):
+    _which = 2
+    _destroy = "ellm_matmul_add_w4_destroy"
+
+    @classmethod
+    def new(cls, ptr1, w4_ptr, scales_ptr, ptr3, output_ptr, m_max, n_max, k_max, group, *, zeros=None, max_batch=None,
+            a_row_stride=0, residual_row_stride=0, output_row_stride=0, device=0, stream=None, async_=False):
+        """output = ptr3 (residual, may be None) + ptr1 [m, k] . W^T, W[n, k] = (q[n, k] - z) * scale with one
+        scale (and zero point) per `group` inputs: w4_ptr uint8 [n, k / 2] as pack_int4 lays it out, scales_ptr
+        bf16 [n, k / group], zeros uint8 [n, k / group] or None (8 everywhere)."""
+        self = object.__new__(cls)
+        self._h = None
+        lib = L.load()
+        for name, t, dtype, width in (("w4_ptr", w4_ptr, "uint8", k_max // 2), ("scales_ptr", scales_ptr, "bfloat16", k_max // max(group, 1)),
+                                      ("zeros", zeros, "uint8", k_max // max(group, 1))):
+            _check_tensor(name, t, dtype, (n_max, width))
+        d = L.MatMulAddW4Desc()
+        d.a, d.a_row_stride, d.w4 = _ptr(ptr1), a_row_stride, _ptr(w4_ptr)
+        d.scales, d.zeros, d.group = _ptr(scales_ptr), _ptr(zeros), group
+        d.residual, d.residual_row_stride = _ptr(ptr3), residual_row_stride
+        d.output, d.output_row_stride = _ptr(output_ptr), output_row_stride
+        d.m_max, d.n_max, d.k_max = m_max, n_max, k_max
+        d.max_batch = m_max if max_batch is None else max_batch
+        d.device, d.stream, d.async_ = device, stream, 1 if async_ else 0
+        handle = C.c_void_p()
+        L.check(lib.ellm_matmul_add_w4_create(C.byref(d), C.byref(handle)))
+        self._lib, self._h, self.desc = lib, handle, d
+        self._keep = (ptr1, w4_ptr, scales_ptr, ptr3, output_ptr, zeros)
+        return self
+
+    def run(self, position_index, position_interval, batch_size, cpu_num=1, thread_id=0):
+        L.check(self._lib.ellm_matmul_add_w4_run(self._h, position_index, position_interval, batch_size, cpu_num,
+                                                 thread_id))
+
+
+def pack_int4(q):
+    """uint8 [n, k] of numbers 0..15 -> uint8 [n, k / 2], input 2i in the low half of byte i."""
+    if q.dim() != 2 or q.shape[1] % 2 or str(q.dtype) != "torch.uint8":
+        raise ValueError("q must be uint8 [n, k] with an even k")
+    return (q[:, 0::2] & 15) | (q[:, 1::2] << 4)
 
 
 def main():

@@ -252,6 +252,49 @@ int ellm_step_graph_launch(ellm_step_graph* graph, void* stream);
 int ellm_step_graph_nodes(const ellm_step_graph* graph, size_t* nodes);   /* kernels recorded */
 int ellm_step_graph_destroy(ellm_step_graph* graph);
 
+/* Modified scores.  After ellm_attn_set_scores every run / run_ragged / run_host of the handle
+ * computes, for the row at absolute position pos of sequence b and query head h, over the keys
+ *     lo <= j < hi,   lo = row_begin[b * row_begin_stride + pos]   (0 when row_begin is NULL)
+ *                     hi = max(pos + 1, prefix_lens[b])            (pos + 1 when prefix_lens is NULL),
+ *                          at most the end of the chunk and max_seq
+ *     s_j = scale * q.k_j
+ *     s_j = softcap * tanh(s_j / softcap)                          (softcap > 0)
+ *     s_j = s_j - slopes[h] * |pos - j|                            (slopes not NULL)
+ * and the softmax over those s_j.  A row whose interval is empty gets zeros and an LSE of -infinity;
+ * keys outside a row's interval are without effect whatever they hold, NaN and infinity included.
+ *   row_begin    documents packed one after the other (the row's own document's first position), a
+ *                sliding window of w keys (pos - w + 1), padding before a sequence (its length), padded
+ *                rows (pos + 1: empty).  Values below 0 count as 0.
+ *   prefix_lens  the first prefix_lens[b] positions are seen by all rows of sequence b, earlier rows
+ *                included; they have to lie in one chunk (a row cannot see keys not yet written).
+ * All arrays are device memory, read by every run; they have to stay valid and may be rewritten between
+ * runs.  The distance is that of positions in the handle's cache.  The struct is copied; s NULL, or one
+ * without any part set, goes back to plain attention.  Not together with ellm_attn_set_shared_prefix
+ * nor ellm_attn_run_window (ELLM_ERR_UNSUPPORTED).  Allocates the table of key ranges on the first call
+ * with row_begin; calls on a handle must not overlap, and graphs captured before the call keep what they
+ * captured.  No counterpart in the reference (src/compiler/mul/attention.rs:69-76 is plain causal). */
+typedef struct ellm_attn_scores {
+    float softcap;               /* 0 = none */
+    const float* slopes;         /* [q_heads] fp32 or NULL */
+    const int32_t* row_begin;    /* [max_batch][row_begin_stride] or NULL */
+    size_t row_begin_stride;     /* elements between sequences, at least max_seq */
+    const int32_t* prefix_lens;  /* [max_batch] or NULL */
+} ellm_attn_scores;
+int ellm_attn_set_scores(ellm_attn* h, const ellm_attn_scores* s);
+
+/* A prefix that all sequences of the batch share (a system prompt, a document under many questions),
+ * kept once: k and v hold its prefix_len rows, element (kv head, row, c) at kvh * kv_head_stride +
+ * row * position_stride + c, bf16 - for instance one sequence's slot of another cache.  Afterwards the
+ * handle's cache and positions count what FOLLOWS the prefix: the row at position p of sequence b
+ * attends all prefix rows and cache rows 0..=p of its sequence (with p = -1 in run_ragged: the prefix
+ * alone).  The prefix is read once for the whole batch, not once per sequence, in decode steps of any
+ * batch.  k NULL or prefix_len 0 removes it.  Not together with ellm_attn_set_scores nor
+ * ellm_attn_run_window (ELLM_ERR_UNSUPPORTED).  May allocate workspace; calls on a handle must not
+ * overlap, and graphs captured before the call keep what they captured.  No counterpart in the
+ * reference (one private K/V buffer per sequence slot, src/memory/cache.rs:69-75). */
+int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size_t kv_head_stride,
+                                size_t position_stride, size_t prefix_len);
+
 /* Counters for the benchmark: kernels launched by this handle since creation, and
  * per-kernel device time when profiling is on (events around each launch). */
 typedef enum ellm_kernel_id {

@@ -119,8 +119,43 @@ int ellm_matmul_add_destroy(ellm_matmul_add* h);
 int ellm_matmul_add_run(ellm_matmul_add* h, size_t position_index, size_t position_interval, size_t batch_size,
                         size_t cpu_num, size_t thread_id);
 
+/* ---- MatMulAddW4: output = residual + A . W^T with 4-bit weights --------------------------------
+ * MatMulAdd for a checkpoint whose weights are 4-bit numbers with one scale per group of inputs:
+ *     W[n][k] = (q[n][k] - z[n][k / group]) * scale[n][k / group],   q in 0..15.
+ * The sum is formed in fp32 and rounded to bf16 once; runs of at most 16 rows multiply by q - z and
+ * apply the scale to the fp32 sums, larger ones multiply by W rounded to bf16.  Weights, scales and
+ * zero points are read by every run, in place; a handle for more than 16 rows keeps a bf16 workspace
+ * of n_max x k_max.  Handles of this kind are `which` 2 of the ellm_matmul_* calls below. */
+typedef struct ellm_matmul_add_w4 ellm_matmul_add_w4;
+
+typedef struct ellm_matmul_add_w4_desc {
+    const void* a;             /* A [m_max x k_max] bf16                                        */
+    size_t a_row_stride;       /* elements; 0 = k_max                                           */
+    const void* w4;            /* [n_max][k_max / 2] bytes: input 2i in the low half of byte i, 2i + 1 in the high half */
+    const void* scales;        /* [n_max][k_max / group] bf16                                   */
+    const void* zeros;         /* [n_max][k_max / group] bytes, 0..127, or NULL = 8 everywhere  */
+    size_t group;              /* 32, 64 or 128                                                 */
+    const void* residual;      /* [m_max x n_max] bf16 or NULL                                  */
+    size_t residual_row_stride; /* elements; 0 = n_max                                          */
+    void* output;              /* [m_max x n_max] bf16; may alias residual                      */
+    size_t output_row_stride;  /* elements; 0 = n_max                                           */
+    size_t m_max;              /* max_interval * max_batch                                      */
+    size_t n_max;              /* a multiple of 8                                               */
+    size_t k_max;              /* a multiple of 128                                             */
+    size_t max_batch;
+    int device;
+    void* stream;
+    int async;
+} ellm_matmul_add_w4_desc;
+
+int ellm_matmul_add_w4_create(const ellm_matmul_add_w4_desc* desc, ellm_matmul_add_w4** out);
+int ellm_matmul_add_w4_destroy(ellm_matmul_add_w4* h);
+int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t position_interval, size_t batch_size,
+                           size_t cpu_num, size_t thread_id);
+
 /* Launches and device time of a handle's kernel since profiling was switched on (events around
- * every launch; for measurement only).  `which`: 0 = ellm_matmul3, 1 = ellm_matmul_add. */
+ * every launch; for measurement only).  `which`: 0 = ellm_matmul3, 1 = ellm_matmul_add,
+ * 2 = ellm_matmul_add_w4. */
 int ellm_matmul_set_profiling(void* handle, int which, int on);
 int ellm_matmul_kernel_stats(void* handle, int which, uint64_t* launches, uint64_t* timed_launches, double* ms);
 /* Waits for the handle's stream and reports a device-side wait that ran out since the last check
