@@ -456,12 +456,14 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
     if (interval > 1) {
         if (h->d.prefill_kernel == ELLM_PREFILL_TCGEN05) use_tc = true;
         else if (h->d.prefill_kernel == ELLM_PREFILL_AUTO) use_tc = ellm::tcgen05_prefers(h->tc, interval, h->group);
-        if (ext) use_tc = false;
+        if (ext)   // (a short chunk leaves most of a 128-row tile empty: the warp-level kernel, as above)
+            use_tc = h->tc.ready_ext && h->d.prefill_kernel != ELLM_PREFILL_WARP_MMA &&
+                     (use_tc || interval * static_cast<size_t>(h->group) >= 16);
     }
     // the chunk's K/V rows go into the cache inside the attention kernel where that is possible (a decode
     // step always does; the tensor-memory prefill kernel when the chunk starts on a key-tile boundary),
     // else by the append kernel first
-    const bool fused = use_tc && do_append && !out_f32 &&
+    const bool fused = use_tc && do_append && !out_f32 && !ext &&
                        ellm::tcgen05_can_fuse_append(h->tc, h->d, positions, position_index, batch, key_begin, key_end);
     // (a decode step whose rows may see nothing would not visit the newest row: appended up front as well)
     const bool decode_appends = !h->prefix_on && !h->mods.row_begin;
@@ -479,11 +481,13 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
                            decode_out_override, h->decode_early != 0 && stream_override == nullptr && !ext);
     } else {
         if (use_tc) {
-            if (!h->tc.ready)
+            if (!h->tc.ready && !ext)
                 return fail(ELLM_ERR_UNSUPPORTED, "tcgen05 prefill unavailable for this handle: %s", h->tc.why);
             {
                 LaunchScope ls(h, ELLM_KERNEL_PREFILL_TCGEN05);
-                rc = ellm::launch_prefill_tcgen05(h->tc, h->d, positions, position_index, interval, batch, key_begin, key_end,
+                rc = ext ? ellm::launch_prefill_tcgen05_ext(h->tc, h->d, h->mods, positions, position_index, interval, batch, lse_out,
+                                                            h->status_dev, h->stream)
+                         : ellm::launch_prefill_tcgen05(h->tc, h->d, positions, position_index, interval, batch, key_begin, key_end,
                                                   out_f32, lse_out, h->status_dev, h->stream, fused);
             }
             if (rc == ELLM_ERR_UNSUPPORTED) return fail(rc, "tcgen05 prefill: %s", h->tc.why);
@@ -589,6 +593,7 @@ int ellm_attn_destroy(ellm_attn* h) {
     cudaFree(h->part_lse);
     cudaFree(h->positions_dev);
     cudaFree(h->status_dev);
+    cudaFree(h->tc.ranges);
     if (h->status_host) cudaFreeHost(h->status_host);
     delete h;
     return ELLM_OK;
@@ -1179,6 +1184,17 @@ int ellm_attn_set_scores(ellm_attn* h, const ellm_attn_scores* s) {
         m.rb_stride = static_cast<long long>(s->row_begin_stride);
         m.prefix_lens = s->prefix_lens;
         m.max_seq = static_cast<long long>(h->d.max_seq);
+        if (s->row_begin && !h->tc.ranges && h->tc.ready_ext) {   // the chunk kernel's key ranges, one per row tile
+            const size_t tile_pos = 128 / static_cast<size_t>(h->group);
+            const size_t tiles = (h->d.max_interval + tile_pos - 1) / tile_pos * h->d.max_batch;
+            DeviceGuard guard(h->d.device);
+            if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", h->d.device);
+            if (cudaMalloc(&h->tc.ranges, tiles * sizeof(int4)) != cudaSuccess) {
+                cudaGetLastError();
+                h->tc.ranges = nullptr;
+                return fail(ELLM_ERR_NO_MEMORY, "allocation of %zu key ranges failed", tiles);
+            }
+        }
     } else if (h->prefix_on) {
         return ELLM_OK;   // nothing to take back
     }

@@ -27,12 +27,22 @@
 // Every wait is bounded (about two seconds): when one runs out the kernel sets a
 // status word, all roles leave their loops, tensor memory is released and the
 // kernel returns; the host turns the status into ELLM_ERR_DEVICE_TIMEOUT.
+//
+// kExt instantiations (score_mods.cuh): scores capped and biased, a key interval per row, key tiles of a
+// shared prefix ahead of the sequence's own, and any group of up to 128 query heads (a row tile holds the
+// floor(128 / G) positions that fit).  An item walks the 128-key tiles from the first to the last key any of
+// its rows sees; tiles that all rows of a row tile see whole take the one-pass step, the others the two-pass
+// step with the interval applied.  The interval hulls come from a table filled by a small kernel ahead
+// of this one (row_begin), or follow from the positions alone.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/ellm_attn.h"
 #include "common.cuh"
+#include "score_mods.cuh"
 
 namespace ellm {
 
@@ -71,6 +81,37 @@ struct Tcgen05Plan {
     int persistent = -1;                                   // ellm_attn_set_option("tc_persistent"): -1 auto, 0 one CTA per item, 1 one CTA per SM
     int fuse_append = 1;                                   // ellm_attn_set_option("tc_fuse_append"): 0 keeps the separate append kernel
     int* sched = nullptr;                                  // the item counter and the exit counter of the one-CTA-per-SM form (the handle's)
+    // kExt: any group of up to 128 heads; the tensor maps of the last such launch and what they depend on
+    bool ready_ext = false;
+    int4* ranges = nullptr;                                // key ranges of every row tile (the handle's), when row_begin is set
+    struct ExtKey {
+        long long kv_rows = -1;
+        size_t interval = 0, batch = 0;
+        const void *pk = nullptr, *pv = nullptr;
+        long long ps1 = 0, ps2 = 0, plen = 0;
+        bool operator==(const ExtKey& o) const {
+            return kv_rows == o.kv_rows && interval == o.interval && batch == o.batch && pk == o.pk && pv == o.pv && ps1 == o.ps1 &&
+                   ps2 == o.ps2 && plen == o.plen;
+        }
+    } ext_key;
+    CUtensorMap ext_q, ext_k, ext_v, ext_pk, ext_pv;
+};
+
+// kExt bits
+enum { kExtOn = 1, kExtCap = 2, kExtBias = 4 };
+
+struct TcExt {
+    ScoreMods mods;
+    const int4* ranges = nullptr;   // [batch][tiles]: (first key, end, last "lo", first "hi") of a row tile's rows; nullptr: from the positions
+    int tile_pos = 0;               // positions per row tile = 128 / group
+    int tiles = 0;                  // row tiles per sequence
+    int prefix_tiles = 0;           // 128-key tiles of the shared prefix
+    float cap_coef[6] = {};         // the tanh polynomial times cap_log2
+    // q and the cache, for the rows recomputed key by key
+    const __nv_bfloat16* q = nullptr;
+    const __nv_bfloat16* k = nullptr;
+    const __nv_bfloat16* v = nullptr;
+    long long s0 = 0, s1 = 0, s2 = 0;
 };
 
 struct TcParams {
@@ -93,6 +134,9 @@ struct TcParams {
     unsigned long long wait_timeout_ns;   // bound of every device-side wait
     int debug_skip_item;    // test hook: ring item (K_0, V_0, K_1, ...) the producer never loads; -1 = none
     float scale_log2;
+};
+struct TcParamsExt : TcParams {   // of the kExt instantiations
+    TcExt ext;
 };
 
 // ---------------------------------------------------------------- PTX wrappers
@@ -256,6 +300,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -314,6 +363,14 @@ struct TcItem {
     int nsteps;
     bool zero_tail;
 };
+// kExt: key tiles of the shared prefix (counted in steps), then own tiles from j0 on; row tile t sees the own
+// keys [flo, fhi) whole.
+struct TcItemExt : TcItem {
+    int np;
+    int flo[kTcTiles], fhi[kTcTiles];
+};
+__device__ __forceinline__ int tc_prefix_tiles(const TcItem&) { return 0; }
+__device__ __forceinline__ int tc_prefix_tiles(const TcItemExt& it) { return it.np; }
 
 // The items are numbered heaviest first: later row tiles have more keys.  When all heads' K/V fit
 // in L2 together the order is heaviest-first over the whole launch, else head by head so that one
@@ -359,6 +416,158 @@ __device__ __forceinline__ void tc_item(const TcParams& p, long long idx, TcItem
     it.zero_tail = p.positions != nullptr && static_cast<long long>(it.j0 + it.nsteps) * kTcKeys > it.key_end;
 }
 
+// kExt: what row tile `tile` of sequence b needs of the sequence's own keys, without a table.
+__device__ __forceinline__ int4 tc_range_of_positions(const TcParamsExt& p, int b, long long base, long long end, int tile) {
+    const long long p0 = base + static_cast<long long>(tile) * p.ext.tile_pos;
+    const long long p1 = min(p0 + p.ext.tile_pos, base + p.interval) - 1;
+    const long long pre = p.ext.mods.prefix_lens ? p.ext.mods.prefix_lens[b] : 0;
+    const long long ke = max(0ll, min(max(p1 + 1, pre), end));
+    long long fhi = p0 < 0 ? 0 : min(max(p0 + 1, pre), end);
+    if (p.ext.mods.slopes) fhi = min(fhi, p0 + 1);   // beyond the position the distance changes sign
+    return make_int4(0, static_cast<int>(ke), 0, static_cast<int>(max(0ll, fhi)));
+}
+
+__device__ __forceinline__ void tc_item(const TcParamsExt& p, long long idx, TcItemExt& it) {
+    {
+        const int heads = p.kv_heads * p.batch;
+        int head;
+        if (p.pair_major) {
+            it.pair = p.pair_tiles - 1 - static_cast<int>(idx / heads);
+            head = static_cast<int>(idx % heads);
+        } else {
+            head = static_cast<int>(idx / p.pair_tiles);
+            it.pair = p.pair_tiles - 1 - static_cast<int>(idx % p.pair_tiles);
+        }
+        it.kvh = head % p.kv_heads;
+        it.b = head / p.kv_heads;
+        it.base = p.positions ? static_cast<long long>(p.positions[it.b]) : p.base;
+        it.key_end = p.positions ? min(it.base + p.interval, p.max_seq) : p.key_end;
+        it.np = p.ext.prefix_tiles;
+        it.lo = 0;
+        int4 r[kTcTiles];
+        int j0 = 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < kTcTiles; ++t) {
+            const int tile = it.pair * kTcTiles + t;
+            r[t] = make_int4(0, 0, 0, 0);
+            if (tile < p.ext.tiles)
+                r[t] = p.ext.ranges ? p.ext.ranges[it.b * p.ext.tiles + tile] : tc_range_of_positions(p, it.b, it.base, it.key_end, tile);
+            if (r[t].x < r[t].y) j0 = min(j0, r[t].x / kTcKeys);
+            it.flo[t] = r[t].z;
+            it.fhi[t] = r[t].w;
+        }
+        it.j0 = j0 == 0x7fffffff ? 0 : j0;
+        it.nsteps = 0;
+#pragma unroll
+        for (int t = 0; t < kTcTiles; ++t) {
+            const bool rows = it.pair * kTcTiles + t < p.ext.tiles;
+            it.steps[t] = rows ? it.np + (r[t].x < r[t].y ? (r[t].y + kTcKeys - 1) / kTcKeys - it.j0 : 0) : 0;
+            it.nsteps = max(it.nsteps, it.steps[t]);
+        }
+        // as in tc_item, for the last own tile (a prefix tile is cut by its tensor map)
+        it.zero_tail = p.positions != nullptr && it.nsteps > it.np &&
+                       static_cast<long long>(it.j0 + it.nsteps - it.np) * kTcKeys > it.key_end;
+    }
+}
+
+// The key ranges of every row tile, from row_begin: one block per (row tile, sequence).
+__global__ void __launch_bounds__(128) tc_ranges_kernel(const ScoreMods m, const int32_t* positions, long long base_all, int interval,
+                                                        long long max_seq, int tile_pos, int tiles, int4* out) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int s[4];   // first key, end, last lo, first hi
+    const int tile = blockIdx.x, b = blockIdx.y;
+    if (threadIdx.x == 0) { s[0] = 0x7fffffff; s[1] = 0; s[2] = 0; s[3] = 0x7fffffff; }
+    __syncthreads();
+    const long long base = positions ? static_cast<long long>(positions[b]) : base_all;
+    const int r = tile * tile_pos + static_cast<int>(threadIdx.x);
+    if (threadIdx.x < tile_pos && r < interval) {
+        const long long pos = base + r;
+        long long lo, hi;
+        row_interval(m, b, pos, min(base + interval, max_seq), lo, hi);
+        if (lo < hi) {
+            atomicMin(&s[0], static_cast<int>(lo));
+            atomicMax(&s[1], static_cast<int>(hi));
+        }
+        atomicMax(&s[2], static_cast<int>(lo));
+        if (m.slopes) hi = min(hi, pos + 1);
+        atomicMin(&s[3], static_cast<int>(max(0ll, hi)));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) out[b * tiles + tile] = s[1] > 0 ? make_int4(s[0], s[1], s[2], s[3]) : make_int4(0, 0, s[2], s[3]);
+}
+
+// kExt: a row's constants for turning products into scores.
+struct TcRow {
+    float scale_log2, cap_in, cap_log2;
+    float slope;     // times log2(e)
+    float dist0;     // position minus the tile's first key
+};
+// One score in log2 units; column c of the tile.
+template <int kExt>
+__device__ __forceinline__ float tc_score(const TcRow& r, float t, int c) {
+    float x = (kExt & kExtCap) ? r.cap_log2 * tanh_any(t * r.cap_in) : t * r.scale_log2;
+    if (kExt & kExtBias) x -= r.slope * fabsf(r.dist0 - static_cast<float>(c));
+    return x;
+}
+// 64 products of one row (columns c0 ..) -> scores in log2 units plus `off`, in place.  kAhead: no column lies
+// beyond the row's position (the distance needs no absolute value).  All lanes of the warp call.
+template <int kExt, bool kAhead>
+__device__ __forceinline__ void tc_scores64(float (&s)[64], const TcRow& r, const float (&coef)[6], int c0, float off) {
+    // (opaque: 64 biases are cheaper computed again in the second pass than kept from the first)
+    float dist0 = r.dist0;
+    asm volatile("" : "+f"(dist0));
+    const float base = (kExt & kExtBias) && kAhead ? off - r.slope * (dist0 - static_cast<float>(c0)) : off;
+    const uint64_t base2 = pack2(base, base);
+    auto add_of = [&](int i) -> uint64_t {   // what is added to scores i, i + 1
+        if constexpr ((kExt & kExtBias) != 0 && kAhead) return pack2(fmaf(r.slope, static_cast<float>(i), base), fmaf(r.slope, static_cast<float>(i + 1), base));
+        else return base2;
+    };
+    bool poly = true;
+    if constexpr ((kExt & kExtCap) != 0) {
+        float m0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), m1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
+#pragma unroll
+        for (int i = 6; i < 62; i += 4) {
+            m0 = max3(m0, fabsf(s[i]), fabsf(s[i + 1]));
+            m1 = max3(m1, fabsf(s[i + 2]), fabsf(s[i + 3]));
+        }
+        m0 = max3(m0, fabsf(s[62]), fabsf(s[63]));
+        poly = __all_sync(0xffffffffu, fmaxf(m0, m1) * r.cap_in <= kTanhPolyMax);
+    }
+    if constexpr ((kExt & kExtCap) == 0) {
+        const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) unpack2(fma2(pack2(s[i], s[i + 1]), scale2, add_of(i)), s[i], s[i + 1]);
+    } else if (poly) {
+        const uint64_t in2 = pack2(r.cap_in, r.cap_in);
+        uint64_t c[6];
+#pragma unroll
+        for (int i = 0; i < 6; ++i) c[i] = pack2(coef[i], coef[i]);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+            const uint64_t u = mul2(pack2(s[i], s[i + 1]), in2), v = mul2(u, u);
+            uint64_t q = fma2(c[5], v, c[4]);
+            q = fma2(q, v, c[3]);
+            q = fma2(q, v, c[2]);
+            q = fma2(q, v, c[1]);
+            q = fma2(q, v, c[0]);
+            unpack2(fma2(u, q, add_of(i)), s[i], s[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+            float a0, a1;
+            unpack2(add_of(i), a0, a1);
+            s[i] = r.cap_log2 * tanh_any(s[i] * r.cap_in) + a0;
+            s[i + 1] = r.cap_log2 * tanh_any(s[i + 1] * r.cap_in) + a1;
+        }
+    }
+    if constexpr ((kExt & kExtBias) != 0 && !kAhead) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] -= r.slope * fabsf(dist0 - static_cast<float>(c0 + i));
+    }
+}
+
 // A wait of the teardown: bounded, sets no status.
 __device__ __noinline__ bool mbar_wait_quiet(uint32_t bar, uint32_t parity, unsigned long long timeout_ns) {
     const unsigned long long t0 = global_timer_ns();
@@ -376,14 +585,18 @@ __device__ __noinline__ bool mbar_wait_quiet(uint32_t bar, uint32_t parity, unsi
 struct TcFixed {
     float m_used, l;
 };
+template <int kExt, class... Ext>
 __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, float scale_log2, float m_used, float l,
-                                                   float first_half_sum, uint32_t* pk) {
+                                                   float first_half_sum, uint32_t* pk, const Ext... ext) {
     float mx = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
         float v[32];
         tmem_ld32(tS + 64 + c * 32, v);
         tmem_wait_ld();
+        if constexpr (kExt != 0)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = tc_score<kExt>(ext..., v[i], 64 + c * 32 + i);
         float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
         for (int i = 6; i < 30; i += 6) {
@@ -394,7 +607,7 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         }
         mx = max3(mx, max3(m0, v[30], v[31]), m1);
     }
-    const float m_new = fmaxf(m_used, mx * scale_log2);
+    const float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * scale_log2);
     // rows whose maximum did not move far keep it (their corr is 1): as in the two-pass step
     const bool moved = m_new - m_used > kTcRescaleThreshold;
     const float corr = moved ? fast_exp2(m_used - m_new) : 1.0f;
@@ -426,9 +639,12 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         float v[32];
         tmem_ld32(tS + 64 + c * 32, v);
         tmem_wait_ld();
+        if constexpr (kExt != 0)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = tc_score<kExt>(ext..., v[i], 64 + c * 32 + i);
 #pragma unroll
         for (int cc = 0; cc < 16; ++cc) {
-            const uint64_t x2 = fma2(pack2(v[2 * cc], v[2 * cc + 1]), scale2, negm2);
+            const uint64_t x2 = kExt != 0 ? add2(pack2(v[2 * cc], v[2 * cc + 1]), negm2) : fma2(pack2(v[2 * cc], v[2 * cc + 1]), scale2, negm2);
             float x0, x1;
             unpack2(x2, x0, x1);
             const uint64_t p2 = pack2(fast_exp2(x0), fast_exp2(x1));
@@ -448,11 +664,14 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
 
 // kFused: the chunk's own K/V rows come from k_new / v_new and are written into the cache here (a
 // separate instantiation, so that the plain kernel carries none of its state).
-template <typename OutT, bool kFused>
+// kExt: modified scores, intervals, shared prefix (map_kn / map_vn are then the prefix's maps).
+template <typename OutT, bool kFused, int kExt = 0>
 __global__ void __launch_bounds__(kTcThreads, 1)
 prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
-                       const __grid_constant__ CUtensorMap map_vn, const TcParams p) {
+                       const __grid_constant__ CUtensorMap map_vn,
+                       const std::conditional_t<kExt != 0, TcParamsExt, TcParams> p) {
+    using Item = std::conditional_t<kExt != 0, TcItemExt, TcItem>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -463,7 +682,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-        if (kFused) {
+        if (kFused || kExt != 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kn) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_vn) : "memory");
         }
@@ -544,7 +763,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint32_t tO = tmem + lane_base + 256 + t * 128;
         int steps_done = 0;     // key steps of this row tile over all items so far
         bool ok = true;
-        TcItem it;
+        Item it;
         int n_traced = 0;
         for (long long k = 0; ok; ++k) {
             int idx = n_items;
@@ -557,9 +776,30 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             tc_item(p, idx, it);
             const int tr = 8 + 8 * n_traced + 4 * t;   // trace slots of this item and tile
             ++n_traced;
-            const int rho = (it.pair * kTcTiles + t) * kTcTileRows + row;
+            int rho = (it.pair * kTcTiles + t) * kTcTileRows + row;
+            if constexpr (kExt != 0)   // a row tile holds whole positions
+                rho = row < p.ext.tile_pos * p.group ? (it.pair * kTcTiles + t) * p.ext.tile_pos * p.group + row : total_rows;
             const bool valid = rho < total_rows;
             const int pos = valid ? rho / p.group : 0, g = valid ? rho % p.group : 0;
+            // kExt: the row's interval of own keys, its constants
+            int row_lo = 0, row_hi = 0;
+            TcRow xr{};
+            float coef[6] = {};
+            if constexpr (kExt != 0) {
+                if (valid) {
+                    long long a, z;
+                    row_interval(p.ext.mods, it.b, it.base + pos, it.key_end, a, z);
+                    row_lo = static_cast<int>(a);
+                    row_hi = static_cast<int>(z);
+                }
+                xr.scale_log2 = p.scale_log2;
+                xr.cap_in = p.ext.mods.cap_in;
+                xr.cap_log2 = p.ext.mods.cap_log2;
+                if ((kExt & kExtBias) && valid) xr.slope = p.ext.mods.slopes[it.kvh * p.group + g] * kLog2e;
+                if constexpr ((kExt & kExtCap) != 0)
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) coef[i] = p.ext.cap_coef[i];
+            }
             const long long lim = valid ? min(it.base + pos, it.key_end - 1) : -1;   // last key this row may see
             const long long tile_min_lim = min(it.base + ((it.pair * kTcTiles + t) * kTcTileRows) / p.group, it.key_end - 1);
             const int my_steps = it.steps[t];
@@ -572,11 +812,25 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (!ok) break;
                 if (j == 0 && (warp & 3) == 0 && lane == 0) TC_TRACE(tr);
                 tc_fence_after();
-                const long long key0 = static_cast<long long>(it.j0 + j) * kTcKeys;
-                const int lo = j == 0 ? it.lo : 0;                     // columns below it lie before the key window
-                const bool edge = key0 + kTcKeys - 1 > tile_min_lim || lo > 0;   // the causal edge (or the window's start) crosses this tile
+                long long key0 = static_cast<long long>(it.j0 + j) * kTcKeys;
+                int lo = j == 0 ? it.lo : 0;                           // columns below it lie before the key window
+                bool edge = key0 + kTcKeys - 1 > tile_min_lim || lo > 0;   // the causal edge (or the window's start) crosses this tile
                 const long long dlim = lim - key0;                     // last column this row may see
-                const int rel = dlim < 0 ? -1 : (dlim > 127 ? 127 : static_cast<int>(dlim));
+                int rel = dlim < 0 ? -1 : (dlim > 127 ? 127 : static_cast<int>(dlim));
+                if constexpr (kExt != 0) {
+                    if (j < it.np) {   // a tile of the shared prefix: seen whole, up to its end
+                        const long long left = p.ext.mods.plen - static_cast<long long>(j) * kTcKeys;
+                        lo = 0;
+                        rel = left < kTcKeys ? static_cast<int>(left) - 1 : kTcKeys - 1;
+                        edge = left < kTcKeys;
+                    } else {
+                        key0 = static_cast<long long>(it.j0 + j - it.np) * kTcKeys;
+                        lo = min(max(row_lo - static_cast<int>(key0), 0), kTcKeys);
+                        rel = min(max(row_hi - static_cast<int>(key0), 0), kTcKeys) - 1;
+                        edge = static_cast<int>(key0) < it.flo[t] || static_cast<int>(key0) + kTcKeys > it.fhi[t];
+                    }
+                    xr.dist0 = static_cast<float>(static_cast<int>(it.base + pos - key0));
+                }
                 // Fast path (every step but the first, unless a score leaps far above the maximum in use):
                 // exponentiate against the maximum already in use, in one pass.  P is held in registers
                 // until the step's row sum has shown that nothing leapt - then it is consistent with O
@@ -596,10 +850,11 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                         tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                         tmem_wait_ld();
+                        if constexpr (kExt != 0) tc_scores64<kExt, true>(s, xr, coef, half * 64, -m_used);
                         uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll
                         for (int cc = 0; cc < 32; ++cc) {
-                            const uint64_t x2 = fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
+                            const uint64_t x2 = kExt != 0 ? pack2(s[2 * cc], s[2 * cc + 1]) : fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
                             uint64_t p2;
                             if (kTcPolyEvery > 0 && (cc % kTcPolyDiv) == kTcPolyDiv - 1) {
                                 p2 = exp2_poly2(x2);
@@ -618,7 +873,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         half_sum[half] = sa + sb;
                         // No row maximum is tracked here.  A score far above the maximum in use shows up as a huge
                         // term of the sum (2^16 and more: one key 16 octaves above, or infinity).
-                        const bool leapt = __any_sync(0xffffffffu, !(half_sum[half] < kTcSumTrigger));
+                        const bool leapt = __any_sync(0xffffffffu, !(half_sum[half] < kTcSumTrigger) && (kExt == 0 || valid));
                         if (half == 0) {
                             if (leapt) {   // S_t is still intact: the whole step the slow way
                                 slow = true;
@@ -628,7 +883,9 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         } else {
                             if (leapt) {   // the first half's P is already in place: bring it and O_t to the new maximum
                                 uint32_t redone[32];   // (addressable only here: pk itself stays in registers)
-                                const TcFixed f = tc_fix_second_half(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone);
+                                TcFixed f;
+                                if constexpr (kExt != 0) f = tc_fix_second_half<kExt>(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone, xr);
+                                else f = tc_fix_second_half<0>(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone);
                                 m_used = f.m_used;
                                 l = f.l;
 #pragma unroll
@@ -655,6 +912,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         tmem_ld32(tS + h * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                         tmem_ld32(tS + h * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                         tmem_wait_ld();
+                        if constexpr (kExt != 0) tc_scores64<kExt, false>(s, xr, coef, h * 64, 0.0f);
                         if (edge) {
 #pragma unroll
                             for (int c = 0; c < 64; ++c) s[c] = (h * 64 + c <= rel && h * 64 + c >= lo) ? s[c] : -INFINITY;
@@ -672,7 +930,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         m1 = max3(m1, s[62], s[63]);
                         mx = max3(mx, fmaxf(m0, m1), fmaxf(m2, m3));
                     }
-                    const float m_new = fmaxf(m_used, mx * p.scale_log2);
+                    const float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * p.scale_log2);
                     // rescale O only when the maximum moved far enough to matter; otherwise keep
                     // exponentiating against the stale maximum (O and l stay consistent with it)
                     const bool need = (m_new - m_used > kTcRescaleThreshold) || (m_used == -INFINITY && m_new != -INFINITY);
@@ -709,6 +967,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                             tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                             tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                             tmem_wait_ld();
+                            if constexpr (kExt != 0) tc_scores64<kExt, false>(s, xr, coef, half * 64, -msub);
                             if (edge) {
 #pragma unroll
                                 for (int c = 0; c < 64; ++c) s[c] = (half * 64 + c <= rel && half * 64 + c >= lo) ? s[c] : -INFINITY;
@@ -717,7 +976,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                             for (int cc = 0; cc < 32; ++cc) {
                                 const int c = half * 32 + cc;
-                                const uint64_t x2 = fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
+                                const uint64_t x2 = kExt != 0 ? pack2(s[2 * cc], s[2 * cc + 1]) : fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
                                 uint64_t p2;
                                 if (kTcPolyEvery > 0 && (c % kTcPolyDiv) == kTcPolyDiv - 1) {
                                     p2 = exp2_poly2(x2);
@@ -753,12 +1012,26 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             OutT* orow = reinterpret_cast<OutT*>(p.out) + row_index * kHeadDim;
             if (my_steps > 0) {
                 tc_fence_after();
-                const float inv = (l > 0.0f) ? 1.0f / l : 0.0f;
+                float inv = (l > 0.0f) ? 1.0f / l : 0.0f;
+                bool bad = false;   // kExt: the row is not finite (see exact_row)
+                if constexpr (kExt != 0) {
+                    if (!(l < INFINITY)) bad = true;
+                }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float o[32];
                     tmem_ld32(tO + c * 32, o);
                     tmem_wait_ld();
+                    if constexpr (kExt != 0) {
+                        if (l == 0.0f) {   // sees nothing: zeros, whatever the masked rows of V were
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                        }
+                        float big = 0.0f;   // 0 * x is 0 for a finite x, NaN otherwise
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) big = fmaf(o[i], 0.0f, big);
+                        bad |= !(big == 0.0f);
+                    }
                     if (valid) {
                         if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
@@ -779,6 +1052,21 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                 }
                 if (valid && p.lse) p.lse[row_index] = (m_used + log2f(l)) * kLn2;
+                if constexpr (kExt != 0 && sizeof(OutT) == 2) {
+                    unsigned redo = __ballot_sync(0xffffffffu, bad && valid);
+                    while (redo) {   // rare: one row at a time, the whole warp on it
+                        const int src = __ffs(redo) - 1;
+                        redo &= redo - 1;
+                        const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_head = it.kvh * p.group + __shfl_sync(0xffffffffu, g, src);
+                        const long long r_index = __shfl_sync(0xffffffffu, row_index, src);
+                        const ScoreMods& m = p.ext.mods;
+                        exact_row(m, p.ext.q + r_index * kHeadDim, p.ext.k + it.b * p.ext.s0 + it.kvh * p.ext.s1,
+                                  p.ext.v + it.b * p.ext.s0 + it.kvh * p.ext.s1, p.ext.s2, m.pk + it.kvh * m.ps1, m.pv + it.kvh * m.ps1,
+                                  it.base + r_pos, __shfl_sync(0xffffffffu, row_lo, src), __shfl_sync(0xffffffffu, row_hi, src),
+                                  m.slopes ? m.slopes[r_head] * kLog2e : 0.0f,
+                                  reinterpret_cast<__nv_bfloat16*>(p.out) + r_index * kHeadDim, p.lse ? p.lse + r_index : nullptr, lane);
+                    }
+                }
                 // the next item's first P.V overwrites O_t: its P is only handed over by these same
                 // threads, after the reads above have completed
                 tc_fence_before();
@@ -822,7 +1110,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 store_pending[slot] = false;
                 return true;
             };
-            TcItem it;
+            Item it;
             for (long long k = 0; ok; ++k) {
                 // this CTA's k-th item: its own block index first, then whatever comes next on the list
                 long long idx = blockIdx.x;
@@ -840,11 +1128,16 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     // the previous item's last Q.K^T of this row tile has finished with the Q tile
                     ok = mbar_wait(bar_q_empty(t), (q_loads[t] & 1) ^ 1, abort_word, p.status, kTcWaitQEmpty, p.wait_timeout_ns);
                     if (!ok) break;
-                    const int rho0 = (it.pair * kTcTiles + t) * kTcTileRows;
-                    mbar_arrive_expect_tx(bar_q(t), kTcTileBytes);
+                    int pos0 = (it.pair * kTcTiles + t) * kTcTileRows / p.group;
+                    uint32_t q_bytes = kTcTileBytes;
+                    if constexpr (kExt != 0) {
+                        pos0 = (it.pair * kTcTiles + t) * p.ext.tile_pos;
+                        q_bytes = static_cast<uint32_t>(p.ext.tile_pos * p.group) * kRowBytes;
+                    }
+                    mbar_arrive_expect_tx(bar_q(t), q_bytes);
                     for (int h = 0; h < 2; ++h)
                         tma_load_5d(smem_base + kTcSmemQ + t * kTcTileBytes + h * kTcHalfBytes, &map_q, bar_q(t), h * 64, 0,
-                                    rho0 / p.group, it.kvh, it.b);
+                                    pos0, it.kvh, it.b);
                     ++q_loads[t];
                 }
                 for (int item = 0; item < 2 * it.nsteps && ok; ++item, ++ring_n) {  // K_0, V_0, K_1, V_1, ...
@@ -879,10 +1172,20 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         }
                     } else {
                         const CUtensorMap* map = (item & 1) ? &map_v : &map_k;
+                        int row0 = key0, seq = it.b;
+                        if constexpr (kExt != 0) {
+                            if ((item >> 1) < it.np) {
+                                map = (item & 1) ? &map_vn : &map_kn;
+                                row0 = (item >> 1) * kTcKeys;
+                                seq = 0;
+                            } else {
+                                row0 -= it.np * kTcKeys;
+                            }
+                        }
                         mbar_arrive_expect_tx(bar_kv_full(slot), kTcTileBytes);
                         for (int h = 0; h < 2; ++h)
                             tma_load_4d(smem_base + kTcSmemRing + slot * kTcTileBytes + h * kTcHalfBytes, map, bar_kv_full(slot),
-                                        h * 64, key0, it.kvh, it.b);
+                                        h * 64, row0, it.kvh, seq);
                     }
                 }
                 if (ok && it.zero_tail && it.nsteps > 0) {
@@ -892,7 +1195,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                    p.wait_timeout_ns);
                     if (ok) {
                         // a 128-byte row of either half holds one key; the swizzle only permutes inside a row
-                        const int first = static_cast<int>(it.key_end - static_cast<long long>(it.j0 + it.nsteps - 1) * kTcKeys);
+                        const int first = static_cast<int>(it.key_end - static_cast<long long>(it.j0 + it.nsteps - tc_prefix_tiles(it) - 1) * kTcKeys);
                         unsigned char* tile = smem + kTcSmemRing + slot * kTcTileBytes;
                         for (int r = first; r < kTcKeys; ++r)
                             for (int h = 0; h < 2; ++h) {
@@ -959,7 +1262,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             int steps_done[kTcTiles] = {0, 0};
             int q_loads[kTcTiles] = {0, 0};
             int tails = 0;
-            TcItem it;
+            Item it;
             for (long long k = 0; ok; ++k) {
                 const int idx = take_item(k, ok, kTcWaitSched);
                 if (!ok) break;
@@ -1065,7 +1368,8 @@ inline void tcgen05_plan_init(Tcgen05Plan& plan, const ellm_attn_desc& d, int sm
     plan.ready = false;
     plan.sm_count = sm_count;
     const size_t group = d.q_heads / d.kv_heads;
-    if (group > 128 || (128 % group) != 0) {
+    plan.ready_ext = false;
+    if (group > 128) {
         snprintf(plan.why, sizeof(plan.why), "query heads per KV head (%zu) must divide 128", group);
         return;
     }
@@ -1084,7 +1388,20 @@ inline void tcgen05_plan_init(Tcgen05Plan& plan, const ellm_attn_desc& d, int sm
                  cudaGetErrorString(cudaGetLastError()));
         return;
     }
+    if (cudaFuncSetAttribute(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtCap>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtBias>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtCap | kExtBias>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess) {
+        snprintf(plan.why, sizeof(plan.why), "cannot reserve %d bytes of shared memory: %s", kTcSmemBytes,
+                 cudaGetErrorString(cudaGetLastError()));
+        return;
+    }
     plan.encode = fn;
+    plan.ready_ext = true;
+    if (128 % group != 0) {   // the plain instantiations pack rows without regard to positions
+        snprintf(plan.why, sizeof(plan.why), "query heads per KV head (%zu) must divide 128", group);
+        return;
+    }
     plan.ready = true;
 }
 
@@ -1232,6 +1549,119 @@ inline int launch_prefill_tcgen05(Tcgen05Plan& plan, const ellm_attn_desc& d, co
         out_f32        ? cudaLaunchKernelEx(&cfg, prefill_tcgen05_kernel<float, false>, map_q, map_k, map_v, map_kn, map_vn, p)
         : fused_append ? cudaLaunchKernelEx(&cfg, prefill_tcgen05_kernel<__nv_bfloat16, true>, map_q, map_k, map_v, map_kn, map_vn, p)
                        : cudaLaunchKernelEx(&cfg, prefill_tcgen05_kernel<__nv_bfloat16, false>, map_q, map_k, map_v, map_kn, map_vn, p);
+    return e == cudaSuccess ? ELLM_OK : ELLM_ERR_CUDA;
+}
+
+// A chunk with modified scores, row intervals or a shared prefix (bf16 result).
+inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d, const ScoreMods& mods, const int32_t* positions,
+                                      size_t position_index, size_t interval, size_t batch, float* lse, int* status,
+                                      cudaStream_t stream) {
+    if (!plan.ready_ext) return ELLM_ERR_UNSUPPORTED;
+    const int group = static_cast<int>(d.q_heads / d.kv_heads);
+    const int tile_pos = 128 / group;
+    long long kv_rows = positions ? static_cast<long long>(d.max_seq) : static_cast<long long>(position_index + interval);
+    kv_rows = std::min(kv_rows, static_cast<long long>(d.max_seq));
+    EncodeTiledFn encode = reinterpret_cast<EncodeTiledFn>(plan.encode);
+    Tcgen05Plan::ExtKey key;
+    key.kv_rows = kv_rows; key.interval = interval; key.batch = batch;
+    key.pk = mods.pk; key.pv = mods.pv; key.ps1 = mods.ps1; key.ps2 = mods.ps2; key.plen = mods.plen;
+    if (!(plan.ext_key == key)) {
+        plan.ext_key = Tcgen05Plan::ExtKey();
+        const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+        {
+            cuuint64_t dims[5] = {128, static_cast<cuuint64_t>(group), interval, d.kv_heads, d.max_batch};
+            cuuint64_t strides[4] = {256, d.max_batch * d.q_heads * 256, static_cast<cuuint64_t>(group) * 256, d.q_heads * 256};
+            cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_pos), 1, 1};
+            if (encode(&plan.ext_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(d.q), dims, strides, box, es,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+                snprintf(plan.why, sizeof(plan.why), "cuTensorMapEncodeTiled(q) failed");
+                return ELLM_ERR_UNSUPPORTED;
+            }
+        }
+        auto kv_map = [&](CUtensorMap* map, const void* base, long long rows, size_t s_pos, size_t s_head, size_t s_seq, size_t seqs) {
+            cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(rows), d.kv_heads, seqs};
+            cuuint64_t strides[3] = {s_pos * 2, s_head * 2, s_seq * 2};
+            cuuint32_t box[4] = {64, 128, 1, 1};
+            return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        };
+        if (!kv_map(&plan.ext_k, d.k_cache, kv_rows, d.kv_strides[2], d.kv_strides[1], d.kv_strides[0], batch) ||
+            !kv_map(&plan.ext_v, d.v_cache, kv_rows, d.kv_strides[2], d.kv_strides[1], d.kv_strides[0], batch) ||
+            (mods.plen > 0 && (!kv_map(&plan.ext_pk, mods.pk, mods.plen, mods.ps2, mods.ps1, mods.ps1, 1) ||
+                               !kv_map(&plan.ext_pv, mods.pv, mods.plen, mods.ps2, mods.ps1, mods.ps1, 1)))) {
+            snprintf(plan.why, sizeof(plan.why), "cuTensorMapEncodeTiled(k/v) failed");
+            return ELLM_ERR_UNSUPPORTED;
+        }
+        if (mods.plen == 0) {   // never read; any valid map will do
+            plan.ext_pk = plan.ext_k;
+            plan.ext_pv = plan.ext_v;
+        }
+        plan.ext_key = key;
+    }
+    TcParamsExt p{};
+    p.out = d.out;
+    p.lse = lse;
+    p.status = status;
+    p.positions = positions;
+    p.base = static_cast<long long>(position_index);
+    p.key_begin = 0;
+    p.key_end = kv_rows;
+    p.max_seq = static_cast<long long>(d.max_seq);
+    p.interval = static_cast<int>(interval);
+    p.batch = static_cast<int>(batch);
+    p.max_batch = static_cast<int>(d.max_batch);
+    p.q_heads = static_cast<int>(d.q_heads);
+    p.kv_heads = static_cast<int>(d.kv_heads);
+    p.group = group;
+    p.wait_timeout_ns = plan.wait_timeout_ns;
+    p.debug_skip_item = plan.debug_skip_item;
+    p.scale_log2 = d.scale * kLog2e;
+    p.ext.mods = mods;
+    p.ext.tile_pos = tile_pos;
+    p.ext.tiles = static_cast<int>((interval + tile_pos - 1) / tile_pos);
+    p.ext.prefix_tiles = static_cast<int>((mods.plen + kTcKeys - 1) / kTcKeys);
+    const float c[6] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4, kTanhC5};
+    for (int i = 0; i < 6; ++i) p.ext.cap_coef[i] = c[i] * mods.cap_log2;
+    p.ext.q = static_cast<const __nv_bfloat16*>(d.q);
+    p.ext.k = static_cast<const __nv_bfloat16*>(d.k_cache);
+    p.ext.v = static_cast<const __nv_bfloat16*>(d.v_cache);
+    p.ext.s0 = d.kv_strides[0]; p.ext.s1 = d.kv_strides[1]; p.ext.s2 = d.kv_strides[2];
+    p.pair_tiles = (p.ext.tiles + kTcTiles - 1) / kTcTiles;
+    const unsigned long long items = static_cast<unsigned long long>(p.pair_tiles) * p.kv_heads * p.batch;
+    if (items > 0x7fffffffull || batch > 65535) {
+        snprintf(plan.why, sizeof(plan.why), "too many row tiles for one launch");
+        return ELLM_ERR_UNSUPPORTED;
+    }
+    p.n_items = static_cast<long long>(items);
+    const bool persistent = plan.sched != nullptr && (plan.persistent < 0 ? true : plan.persistent != 0);
+    p.sched = persistent ? plan.sched : nullptr;
+    const unsigned long long kv_bytes = 2ull * (static_cast<unsigned long long>(kv_rows) * batch + mods.plen) * 256ull * d.kv_heads;
+    p.pair_major = kv_bytes <= (96ull << 20) ? 1 : 0;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (mods.row_begin) {
+        p.ext.ranges = plan.ranges;
+        cfg.gridDim = dim3(static_cast<unsigned>(p.ext.tiles), static_cast<unsigned>(batch));
+        cfg.blockDim = dim3(128);
+        if (cudaLaunchKernelEx(&cfg, tc_ranges_kernel, mods, positions, p.base, p.interval, p.max_seq, tile_pos, p.ext.tiles, plan.ranges) != cudaSuccess)
+            return ELLM_ERR_CUDA;
+    }
+    cfg.gridDim = dim3(static_cast<unsigned>(persistent ? std::min<unsigned long long>(items, static_cast<unsigned long long>(plan.sm_count)) : items));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = kTcSmemBytes;
+    auto launch = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, plan.ext_q, plan.ext_k, plan.ext_v, plan.ext_pk, plan.ext_pv, p); };
+    const bool cap = mods.cap_log2 != 0.0f, bias = mods.slopes != nullptr;
+    const cudaError_t e = cap && bias ? launch(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtCap | kExtBias>)
+                          : cap       ? launch(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtCap>)
+                          : bias      ? launch(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn | kExtBias>)
+                                      : launch(prefill_tcgen05_kernel<__nv_bfloat16, false, kExtOn>);
     return e == cudaSuccess ? ELLM_OK : ELLM_ERR_CUDA;
 }
 

@@ -52,6 +52,10 @@ __device__ __forceinline__ float fast_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+// coefficients of u, u^3, ..., u^11 of the polynomial for |u| <= kTanhPolyMax
+constexpr float kTanhPolyMax = 1.0f;
+constexpr float kTanhC0 = 0.9999994040f, kTanhC1 = -0.3332904279f, kTanhC2 = 0.1328143328f, kTanhC3 = -0.0516056642f,
+                kTanhC4 = 0.0167431068f, kTanhC5 = -0.0030670569f;
 // tanh of any argument (saturates through e^(2u) = 0 and infinity; NaN stays NaN)
 __device__ __forceinline__ float tanh_any(float u) {
     const float v = u * u;
@@ -71,7 +75,7 @@ __device__ __forceinline__ float mod_score(const ScoreMods& m, float t, float sl
 // is not finite is recomputed here, so that what a masked key holds never shows.  If the row itself sees
 // a NaN the result stays NaN (and the walk stops once every column is).  All 32 lanes call with the same
 // arguments; lane = 4 consecutive channels.
-__device__ __noinline__ void exact_row(const ScoreMods& m, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+__device__ __noinline__ void exact_row(const ScoreMods m, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
                                        long long s2, const __nv_bfloat16* pk, const __nv_bfloat16* pv, long long pos, long long lo,
                                        long long hi, float slope_log2, __nv_bfloat16* out, float* lse, int lane) {
     float qf[4];
