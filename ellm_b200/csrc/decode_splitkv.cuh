@@ -71,6 +71,11 @@ struct DecodeParams {
     // Only what that kernel cannot have written is touched early: the positions, and cache rows
     // below each sequence's newest row; the queries and the stages that hold a newest row wait.
     int early = 0;
+    // The shared-prefix part of the step, for the merge: pre_parts partials [pre_rows, 128] and [pre_rows]
+    const float* pre_o = nullptr;
+    const float* pre_lse = nullptr;
+    long long pre_rows = 0;
+    int pre_parts = 0;
     // kMods instantiations: capped / biased scores, keys from row_begin[b][position] on (key_begin is 0)
     ScoreMods mods;
 };

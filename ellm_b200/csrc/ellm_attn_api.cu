@@ -161,6 +161,8 @@ struct ellm_attn {
     ellm::Tcgen05Plan tc;              // tensor maps etc. of the tcgen05 prefill kernel
     ellm::ScoreMods mods;              // ellm_attn_set_scores / ellm_attn_set_shared_prefix
     bool scores_on = false, prefix_on = false;
+    float* pre_part = nullptr;         // shared prefix, decode steps: partial O [pre_slots][128], then partial LSE [pre_slots]
+    size_t pre_slots = 0;
     std::mutex mu;
     uint64_t launches[ELLM_KERNEL_COUNT] = {};
     uint64_t timed[ELLM_KERNEL_COUNT] = {};
@@ -265,8 +267,8 @@ int launch_append(ellm_attn* h, cudaStream_t stream, void* k_cache, void* v_cach
 // the light shape (2 warps per row, tables in dynamic shared memory), few rows with many pieces the
 // wide one.  A row's pieces are at most the decode grid's CTAs.
 cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blocks, float* out_f32, void* out_bf16,
-                         float* lse_out, cudaStream_t stream, bool dependent, bool mods = false) {
-    const int pieces_cap = std::min(p.num_ctas, ellm::kMergeMaxPieces);
+                         float* lse_out, cudaStream_t stream, bool dependent, int kind = ellm::kMergePlain) {
+    const int pieces_cap = std::min(p.num_ctas + (kind == ellm::kMergePrefix ? p.pre_parts : 0), ellm::kMergeMaxPieces);
     const size_t smem = ellm::merge_smem_bytes(static_cast<int>(batch), pieces_cap);
     const bool light = blocks >= 128;
     cudaLaunchConfig_t cfg = {};
@@ -280,9 +282,12 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 1 : 0;
     __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out_bf16);
-    if (mods)   // (the pieces of a row follow from its own first key)
-        return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, true>, p, ob, lse_out, pieces_cap)
-                     : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, true>, p, ob, lse_out, pieces_cap);
+    if (kind == ellm::kMergeMods)
+        return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, ellm::kMergeMods>, p, ob, lse_out, pieces_cap)
+                     : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, ellm::kMergeMods>, p, ob, lse_out, pieces_cap);
+    if (kind == ellm::kMergePrefix)
+        return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap)
+                     : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap);
     if (out_f32)
         return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 2, 4>, p, out_f32, lse_out, pieces_cap)
                      : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 8, 10>, p, out_f32, lse_out, pieces_cap);
@@ -320,6 +325,19 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
     p.scale_log2 = h->d.scale * ellm::kLog2e;
     p.num_ctas = h->dec_ctas;
     p.mods = h->mods;
+    if (h->prefix_on) {
+        // the prefix's part first; the own keys' kernel and the merge follow
+        const int splits = ellm::prefix_splits(h->tc, batch, h->d.q_heads, h->d.kv_heads, (h->mods.plen + ellm::kTcKeys - 1) / ellm::kTcKeys);
+        p.pre_rows = static_cast<long long>(batch * h->d.q_heads);
+        p.pre_parts = splits;
+        p.pre_o = h->pre_part;
+        p.pre_lse = h->pre_part + h->pre_slots * ellm::kHeadDim;
+        LaunchScope ls(h, ELLM_KERNEL_PREFILL_TCGEN05);
+        const int rc = ellm::launch_prefix_split(h->tc, h->d, h->mods, batch, splits, h->pre_part, h->pre_part + h->pre_slots * ellm::kHeadDim,
+                                                 h->status_dev, h->stream);
+        if (rc == ELLM_ERR_UNSUPPORTED) return fail(rc, "shared prefix: %s", h->tc.why);
+        if (rc) return fail(rc, "shared prefix launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+    }
     if (append) {   // the new token's K/V rows ride along with the decode kernel
         p.k_new = static_cast<const __nv_bfloat16*>(h->d.k_new);
         p.v_new = static_cast<const __nv_bfloat16*>(h->d.v_new);
@@ -345,7 +363,8 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
         // its first instruction waits for the decode grid's memory to be visible
         LaunchScope ls(h, ELLM_KERNEL_MERGE);
         const cudaError_t e = launch_merge(p, batch, blocks, out_f32, out_f32 ? nullptr : (out_override ? out_override : h->d.out),
-                                           lse_out, h->stream, true, h->scores_on);
+                                           lse_out, h->stream, true,
+                                           h->prefix_on ? ellm::kMergePrefix : h->scores_on ? ellm::kMergeMods : ellm::kMergePlain);
         if (e != cudaSuccess) return fail(ELLM_ERR_CUDA, "merge launch failed: %s", cudaGetErrorString(e));
     }
     ELLM_CUDA(cudaGetLastError());
@@ -466,13 +485,14 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
     const bool fused = use_tc && do_append && !out_f32 && !ext &&
                        ellm::tcgen05_can_fuse_append(h->tc, h->d, positions, position_index, batch, key_begin, key_end);
     // (a decode step whose rows may see nothing would not visit the newest row: appended up front as well)
-    const bool decode_appends = !h->prefix_on && !h->mods.row_begin;
+    const bool prefix_warp = h->prefix_on && !h->tc.ready_ext;   // more than 128 query heads per KV head
+    const bool decode_appends = !prefix_warp && !h->mods.row_begin;
     if (do_append && (interval > 1 || !decode_appends) && !fused) {
         rc = launch_append(h, h->stream, h->d.k_cache, h->d.v_cache, h->d.k_new, h->d.v_new, h->d.kv_strides,
                            h->d.max_batch, h->d.kv_heads, h->d.max_seq, position_index, positions, interval, batch);
         if (rc) return rc;
     }
-    if (interval == 1 && h->prefix_on) {
+    if (interval == 1 && prefix_warp) {
         rc = launch_prefill_warp_mma(h, positions, position_index, interval, batch, key_begin, key_end, nullptr, lse_out, decode_out_override);
     } else if (interval == 1) {
         // early streaming only where the caller vouched for it, and never for a step whose inputs the
@@ -497,7 +517,7 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
         }
     }
     if (rc) return rc;
-    if (h->status_dev && !no_sync && interval > 1)
+    if (h->status_dev && !no_sync && (interval > 1 || h->prefix_on))
         cudaMemcpyAsync(h->status_host, h->status_dev, sizeof(int), cudaMemcpyDeviceToHost, h->stream);
     return finish(h, no_sync);
 }
@@ -594,6 +614,7 @@ int ellm_attn_destroy(ellm_attn* h) {
     cudaFree(h->positions_dev);
     cudaFree(h->status_dev);
     cudaFree(h->tc.ranges);
+    cudaFree(h->pre_part);
     if (h->status_host) cudaFreeHost(h->status_host);
     delete h;
     return ELLM_OK;
@@ -783,8 +804,14 @@ int ellm_attn_run_host(ellm_attn* h, const void* q_host, const void* k_new_host,
         }
         ELLM_CUDA(cudaGraphLaunch(h->graph_exec, run_stream));
         for (int i = 0; i < ELLM_KERNEL_COUNT; ++i) h->launches[i] += h->graph_launches[i];
+        if (h->graph_launches[ELLM_KERNEL_PREFILL_TCGEN05] == 0) {
+            ELLM_CUDA(cudaStreamSynchronize(run_stream));
+            return ELLM_OK;
+        }
+        // a step over a shared prefix: its kernel has device-side waits that can run out
+        ELLM_CUDA(cudaMemcpyAsync(h->status_host, h->status_dev, sizeof(int), cudaMemcpyDeviceToHost, run_stream));
         ELLM_CUDA(cudaStreamSynchronize(run_stream));
-        return ELLM_OK;
+        return finish(h, false);
     }
 
     int rc = enqueue(h->stream);
@@ -1230,6 +1257,19 @@ int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size
     m.ps1 = static_cast<long long>(kv_head_stride);
     m.ps2 = static_cast<long long>(position_stride);
     m.plen = static_cast<long long>(prefix_len);
+    if (!h->pre_part && h->tc.ready_ext) {   // one partial row per (run of prefix tiles, query row), for any batch and prefix length
+        size_t slots = 0;
+        for (size_t b = 1; b <= h->d.max_batch; ++b)
+            slots = std::max(slots, b * h->d.q_heads * ellm::prefix_splits(h->tc, b, h->d.q_heads, h->d.kv_heads, INT64_MAX));
+        DeviceGuard guard(h->d.device);
+        if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", h->d.device);
+        if (cudaMalloc(&h->pre_part, slots * (ellm::kHeadDim + 1) * sizeof(float)) != cudaSuccess) {
+            cudaGetLastError();
+            h->pre_part = nullptr;
+            return fail(ELLM_ERR_NO_MEMORY, "workspace allocation failed (%zu partial rows)", slots);
+        }
+        h->pre_slots = slots;
+    }
     h->mods = m;
     h->prefix_on = true;
     drop_host_step(h);

@@ -49,7 +49,10 @@ __host__ __device__ inline size_t merge_smem_bytes(int batch, int pieces_cap) {
     return (static_cast<size_t>(2 * batch + 1) + static_cast<size_t>(pieces_cap)) * 4;
 }
 
-template <typename OutT, int kWarps, int kAhead, bool kMods = false>
+// kKind: kMergePlain, kMergeMods (the sequences' keys start at row_begin), kMergePrefix (the step has a shared
+// prefix, whose partials - one per run of prefix tiles, of all rows - are further pieces of every row).
+enum { kMergePlain = 0, kMergeMods = 1, kMergePrefix = 2 };
+template <typename OutT, int kWarps, int kAhead, int kKind = kMergePlain>
 // (both shapes are held to 64 registers: they have to fit beside two decode CTAs of ~184 registers x 128 threads -
 // one wide CTA, or the light shape's three or four per SM - or they cannot move in, and release their own
 // dependents, before the decode grid has drained)
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
     // Where this row's pieces are follows from the positions alone, which are older than the decode
     // grid (it lets this grid start only after its own wait): the tile table is rebuilt here, before
     // the wait for the decode grid's results, instead of being read from it afterwards.
-    dec_build_prefix<kMods>(p, s_prefix, s_lens);
+    dec_build_prefix<kKind == kMergeMods>(p, s_prefix, s_lens);
     const long long row = blockIdx.x;
     const int b = static_cast<int>(row / p.q_heads), qh = static_cast<int>(row % p.q_heads);
     const int kvh = qh / p.group, g = qh % p.group, gt = g / 16, r = g % 16;
@@ -92,14 +95,24 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
             c_last = cta_of_tile(total, p.num_ctas, t0 + tiles_b - 1);
         }
     }
-    const int pieces = static_cast<int>(c_last - c_first + 1);
+    const int own_pieces = static_cast<int>(c_last - c_first + 1);
+    const int pieces = own_pieces + (kKind == kMergePrefix ? p.pre_parts : 0);
     const float* lse_base = p.part_lse + (c_first + segment) * 16 + r;            // piece i at + i * 16
     const float* o_base = p.part_o + ((c_first + segment) * 16 + r) * kHeadDim + lane * 4;   // piece i at + i * 16 * 128
+    auto piece_o = [&](int i) -> const float* {
+        if (kKind == kMergePrefix && i >= own_pieces)
+            return p.pre_o + ((i - own_pieces) * p.pre_rows + row) * kHeadDim + lane * 4;
+        return o_base + static_cast<long long>(i) * 16 * kHeadDim;
+    };
+    auto piece_lse_at = [&](int i) -> const float* {
+        if (kKind == kMergePrefix && i >= own_pieces) return p.pre_lse + (i - own_pieces) * p.pre_rows + row;
+        return lse_base + static_cast<long long>(i) * 16;
+    };
     // under a programmatic dependent launch: wait until the decode grid's writes are visible
     // (a no-op for an ordinary launch)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     ct.waited();
-    if (tiles_b == 0) {  // no key in range for this sequence
+    if (pieces == 0) {  // no key in range for this sequence
         if (warp == 0) {
             store_row4<OutT>(orow, make_float4(0.f, 0.f, 0.f, 0.f));
             if (lse && lane == 0) lse[row] = -INFINITY;
@@ -114,13 +127,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
         const int i = warp + u * kWarps;
-        x[u] = i < pieces ? *reinterpret_cast<const float4*>(o_base + static_cast<long long>(i) * 16 * kHeadDim)
+        x[u] = i < pieces ? *reinterpret_cast<const float4*>(piece_o(i))
                           : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     // 1. the maximum of the pieces' log-sum-exps (every piece has seen at least one key: finite)
     float mx = -INFINITY;
     for (int i = threadIdx.x; i < pieces; i += kThreads) {
-        const float l = lse_base[static_cast<long long>(i) * 16];
+        const float l = *piece_lse_at(i);
         if (i < pieces_cap) s_l[i] = l;
         mx = fmaxf(mx, l);
     }
@@ -135,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
     // 2. weighted sums, pieces round-robin over the warps
     float wsum = 0.0f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto piece_lse = [&](int i) { return i < pieces_cap ? s_l[i] : lse_base[static_cast<long long>(i) * 16]; };
+    auto piece_lse = [&](int i) { return i < pieces_cap ? s_l[i] : *piece_lse_at(i); };
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
         const int i = warp + u * kWarps;
@@ -146,7 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merg
         }
     }
     for (int i = warp + kAhead * kWarps; i < pieces; i += kWarps) {   // more pieces than the warps hold ahead
-        const float4 y = *reinterpret_cast<const float4*>(o_base + static_cast<long long>(i) * 16 * kHeadDim);
+        const float4 y = *reinterpret_cast<const float4*>(piece_o(i));
         const float w = __expf(piece_lse(i) - mm);
         wsum += w;
         acc.x += w * y.x; acc.y += w * y.y; acc.z += w * y.z; acc.w += w * y.w;

@@ -34,6 +34,12 @@
 // its rows sees; tiles that all rows of a row tile see whole take the one-pass step, the others the two-pass
 // step with the interval applied.  The interval hulls come from a table filled by a small kernel ahead
 // of this one (row_begin), or follow from the positions alone.
+//
+// kExtSplit: the shared-prefix part of a decode step.  The rows are the step's query rows (chunk row =
+// sequence), the keys the prefix alone, cut into `splits` runs of tiles so that every SM has work, and the
+// result is one fp32 partial (O, LSE) per run; the sequences' own keys go through the split-KV kernel and its
+// merge takes these partials in.  The prefix is read once per 256 query rows of a KV head instead of once per
+// sequence: with 64 sequences on 32768 keys the kernel is bound by the tensor core, with a handful by HBM.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -98,7 +104,7 @@ struct Tcgen05Plan {
 };
 
 // kExt bits
-enum { kExtOn = 1, kExtCap = 2, kExtBias = 4 };
+enum { kExtOn = 1, kExtCap = 2, kExtBias = 4, kExtSplit = 8 };
 
 struct TcExt {
     ScoreMods mods;
@@ -106,6 +112,8 @@ struct TcExt {
     int tile_pos = 0;               // positions per row tile = 128 / group
     int tiles = 0;                  // row tiles per sequence
     int prefix_tiles = 0;           // 128-key tiles of the shared prefix
+    int splits = 1;                 // kExtSplit: runs of prefix tiles, each with its own partial result
+    long long part_rows = 0;        // kExtSplit: rows of one partial
     float cap_coef[6] = {};         // the tanh polynomial times cap_log2
     // q and the cache, for the rows recomputed key by key
     const __nv_bfloat16* q = nullptr;
@@ -367,6 +375,7 @@ struct TcItem {
 // keys [flo, fhi) whole.
 struct TcItemExt : TcItem {
     int np;
+    int p0 = 0, split = 0;   // kExtSplit: first prefix tile of the item's run
     int flo[kTcTiles], fhi[kTcTiles];
 };
 __device__ __forceinline__ int tc_prefix_tiles(const TcItem&) { return 0; }
@@ -467,6 +476,30 @@ __device__ __forceinline__ void tc_item(const TcParamsExt& p, long long idx, TcI
         // as in tc_item, for the last own tile (a prefix tile is cut by its tensor map)
         it.zero_tail = p.positions != nullptr && it.nsteps > it.np &&
                        static_cast<long long>(it.j0 + it.nsteps - it.np) * kTcKeys > it.key_end;
+    }
+}
+
+struct TcItemSplit : TcItemExt {};
+__device__ __forceinline__ void tc_item(const TcParamsExt& p, long long idx, TcItemSplit& it) {
+    // the runs of one (row pair, head) first, so that the items running together share a head's keys in L2
+    it.split = static_cast<int>(idx % p.ext.splits);
+    const int rest = static_cast<int>(idx / p.ext.splits);
+    it.pair = rest % p.pair_tiles;
+    it.kvh = rest / p.pair_tiles;
+    it.b = 0;
+    it.base = 0;
+    it.key_end = 0;
+    it.lo = 0;
+    it.j0 = 0;
+    it.zero_tail = false;
+    long long a = 0, z = 0;
+    assign_range(p.ext.prefix_tiles, p.ext.splits, it.split, &a, &z);
+    it.p0 = static_cast<int>(a);
+    it.np = it.nsteps = static_cast<int>(z - a);
+#pragma unroll
+    for (int t = 0; t < kTcTiles; ++t) {
+        it.steps[t] = it.pair * kTcTiles + t < p.ext.tiles ? it.np : 0;
+        it.flo[t] = it.fhi[t] = 0;
     }
 }
 
@@ -671,7 +704,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
                        const __grid_constant__ CUtensorMap map_vn,
                        const std::conditional_t<kExt != 0, TcParamsExt, TcParams> p) {
-    using Item = std::conditional_t<kExt != 0, TcItemExt, TcItem>;
+    using Item = std::conditional_t<(kExt & kExtSplit) != 0, TcItemSplit, std::conditional_t<kExt != 0, TcItemExt, TcItem>>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -786,7 +819,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             TcRow xr{};
             float coef[6] = {};
             if constexpr (kExt != 0) {
-                if (valid) {
+                if ((kExt & kExtSplit) == 0 && valid) {
                     long long a, z;
                     row_interval(p.ext.mods, it.b, it.base + pos, it.key_end, a, z);
                     row_lo = static_cast<int>(a);
@@ -803,7 +836,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const long long lim = valid ? min(it.base + pos, it.key_end - 1) : -1;   // last key this row may see
             const long long tile_min_lim = min(it.base + ((it.pair * kTcTiles + t) * kTcTileRows) / p.group, it.key_end - 1);
             const int my_steps = it.steps[t];
-            const long long row_index = (static_cast<long long>(pos) * p.max_batch + it.b) * p.q_heads + it.kvh * p.group + g;
+            long long row_index = (static_cast<long long>(pos) * p.max_batch + it.b) * p.q_heads + it.kvh * p.group + g;
+            if constexpr ((kExt & kExtSplit) != 0) row_index += it.split * p.ext.part_rows;
             float m_used = -INFINITY, l = 0.0f;
             for (int j = 0; j < my_steps && ok; ++j) {
                 // lane 0 polls the barrier, the warp follows (32 pollers per warp only add shared-memory traffic)
@@ -819,7 +853,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 int rel = dlim < 0 ? -1 : (dlim > 127 ? 127 : static_cast<int>(dlim));
                 if constexpr (kExt != 0) {
                     if (j < it.np) {   // a tile of the shared prefix: seen whole, up to its end
-                        const long long left = p.ext.mods.plen - static_cast<long long>(j) * kTcKeys;
+                        const long long left = p.ext.mods.plen - static_cast<long long>(it.p0 + j) * kTcKeys;
                         lo = 0;
                         rel = left < kTcKeys ? static_cast<int>(left) - 1 : kTcKeys - 1;
                         edge = left < kTcKeys;
@@ -1176,7 +1210,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         if constexpr (kExt != 0) {
                             if ((item >> 1) < it.np) {
                                 map = (item & 1) ? &map_vn : &map_kn;
-                                row0 = (item >> 1) * kTcKeys;
+                                row0 = (it.p0 + (item >> 1)) * kTcKeys;
                                 seq = 0;
                             } else {
                                 row0 -= it.np * kTcKeys;
@@ -1396,6 +1430,11 @@ inline void tcgen05_plan_init(Tcgen05Plan& plan, const ellm_attn_desc& d, int sm
                  cudaGetErrorString(cudaGetLastError()));
         return;
     }
+    if (cudaFuncSetAttribute(prefill_tcgen05_kernel<float, false, kExtOn | kExtSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmemBytes) != cudaSuccess) {
+        snprintf(plan.why, sizeof(plan.why), "cannot reserve %d bytes of shared memory: %s", kTcSmemBytes,
+                 cudaGetErrorString(cudaGetLastError()));
+        return;
+    }
     plan.encode = fn;
     plan.ready_ext = true;
     if (128 % group != 0) {   // the plain instantiations pack rows without regard to positions
@@ -1552,6 +1591,89 @@ inline int launch_prefill_tcgen05(Tcgen05Plan& plan, const ellm_attn_desc& d, co
     return e == cudaSuccess ? ELLM_OK : ELLM_ERR_CUDA;
 }
 
+// A K or V tensor map: boxes of 128 rows x 64 columns.
+inline bool tcgen05_kv_map(const Tcgen05Plan& plan, CUtensorMap* map, const void* base, long long rows, size_t heads, size_t s_pos,
+                           size_t s_head, size_t s_seq, size_t seqs) {
+    cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(rows), heads, seqs};
+    cuuint64_t strides[3] = {s_pos * 2, s_head * 2, s_seq * 2};
+    cuuint32_t box[4] = {64, 128, 1, 1};
+    cuuint32_t es[4] = {1, 1, 1, 1};
+    return reinterpret_cast<EncodeTiledFn>(plan.encode)(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+                                                        es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Runs of prefix tiles a decode step of `batch` sequences is cut into: one CTA per SM over all row pairs and heads.
+inline int prefix_splits(const Tcgen05Plan& plan, size_t batch, size_t q_heads, size_t kv_heads, long long prefix_tiles) {
+    const size_t tile_pos = 128 / (q_heads / kv_heads);
+    const size_t pairs = (batch + kTcTiles * tile_pos - 1) / (kTcTiles * tile_pos);
+    const long long s = static_cast<long long>(plan.sm_count / (pairs * kv_heads));
+    return static_cast<int>(std::max(1ll, std::min(s, prefix_tiles)));
+}
+
+// The shared-prefix part of a decode step: part_o [splits][batch * q_heads][128] fp32, part_lse [splits][batch * q_heads].
+inline int launch_prefix_split(Tcgen05Plan& plan, const ellm_attn_desc& d, const ScoreMods& mods, size_t batch, int splits, float* part_o,
+                               float* part_lse, int* status, cudaStream_t stream) {
+    const int group = static_cast<int>(d.q_heads / d.kv_heads);
+    const int tile_pos = 128 / group;
+    Tcgen05Plan::ExtKey key;
+    key.batch = batch;
+    key.pk = mods.pk; key.pv = mods.pv; key.ps1 = mods.ps1; key.ps2 = mods.ps2; key.plen = mods.plen;
+    if (!(plan.ext_key == key)) {
+        plan.ext_key = Tcgen05Plan::ExtKey();
+        // the query rows of the step as a chunk of `batch` positions of one sequence
+        cuuint64_t dims[5] = {128, static_cast<cuuint64_t>(group), batch, d.kv_heads, 1};
+        cuuint64_t strides[4] = {256, d.q_heads * 256, static_cast<cuuint64_t>(group) * 256, d.q_heads * 256};
+        cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_pos), 1, 1};
+        cuuint32_t es[5] = {1, 1, 1, 1, 1};
+        if (reinterpret_cast<EncodeTiledFn>(plan.encode)(&plan.ext_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(d.q), dims, strides,
+                                                         box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+            !tcgen05_kv_map(plan, &plan.ext_pk, mods.pk, mods.plen, d.kv_heads, mods.ps2, mods.ps1, mods.ps1, 1) ||
+            !tcgen05_kv_map(plan, &plan.ext_pv, mods.pv, mods.plen, d.kv_heads, mods.ps2, mods.ps1, mods.ps1, 1)) {
+            snprintf(plan.why, sizeof(plan.why), "cuTensorMapEncodeTiled failed");
+            return ELLM_ERR_UNSUPPORTED;
+        }
+        plan.ext_key = key;
+    }
+    TcParamsExt p{};
+    p.out = part_o;
+    p.lse = part_lse;
+    p.status = status;
+    p.interval = static_cast<int>(batch);
+    p.batch = p.max_batch = 1;
+    p.q_heads = static_cast<int>(d.q_heads);
+    p.kv_heads = static_cast<int>(d.kv_heads);
+    p.group = group;
+    p.wait_timeout_ns = plan.wait_timeout_ns;
+    p.debug_skip_item = plan.debug_skip_item;
+    p.scale_log2 = d.scale * kLog2e;
+    p.ext.mods = mods;
+    p.ext.tile_pos = tile_pos;
+    p.ext.tiles = static_cast<int>((batch + tile_pos - 1) / tile_pos);
+    p.ext.prefix_tiles = static_cast<int>((mods.plen + kTcKeys - 1) / kTcKeys);
+    p.ext.splits = splits;
+    p.ext.part_rows = static_cast<long long>(batch * d.q_heads);
+    p.pair_tiles = (p.ext.tiles + kTcTiles - 1) / kTcTiles;
+    p.n_items = static_cast<long long>(p.pair_tiles) * p.kv_heads * splits;
+    if (p.n_items > 0x7fffffffll) return ELLM_ERR_UNSUPPORTED;
+    const bool persistent = plan.sched != nullptr && plan.persistent != 0;
+    p.sched = persistent ? plan.sched : nullptr;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(persistent ? std::min<long long>(p.n_items, plan.sm_count) : p.n_items));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = kTcSmemBytes;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_tcgen05_kernel<float, false, kExtOn | kExtSplit>, plan.ext_q, plan.ext_pk,
+                                             plan.ext_pv, plan.ext_pk, plan.ext_pv, p);
+    return e == cudaSuccess ? ELLM_OK : ELLM_ERR_CUDA;
+}
+
 // A chunk with modified scores, row intervals or a shared prefix (bf16 result).
 inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d, const ScoreMods& mods, const int32_t* positions,
                                       size_t position_index, size_t interval, size_t batch, float* lse, int* status,
@@ -1580,12 +1702,7 @@ inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d
             }
         }
         auto kv_map = [&](CUtensorMap* map, const void* base, long long rows, size_t s_pos, size_t s_head, size_t s_seq, size_t seqs) {
-            cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(rows), d.kv_heads, seqs};
-            cuuint64_t strides[3] = {s_pos * 2, s_head * 2, s_seq * 2};
-            cuuint32_t box[4] = {64, 128, 1, 1};
-            return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            return tcgen05_kv_map(plan, map, base, rows, d.kv_heads, s_pos, s_head, s_seq, seqs);
         };
         if (!kv_map(&plan.ext_k, d.k_cache, kv_rows, d.kv_strides[2], d.kv_strides[1], d.kv_strides[0], batch) ||
             !kv_map(&plan.ext_v, d.v_cache, kv_rows, d.kv_strides[2], d.kv_strides[1], d.kv_strides[0], batch) ||
