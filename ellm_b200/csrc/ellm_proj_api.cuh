@@ -510,19 +510,27 @@ int ellm_matmul_add_run(ellm_matmul_add* h, size_t position_index, size_t positi
 namespace {
 
 typedef void (*W4Kernel)(const ellm::W4Params);
-template <int CB, int NB>
-W4Kernel w4_kernel_of(size_t group) {
-    return group == 128 ? ellm::proj_w4_kernel<CB, NB, 4> : group == 64 ? ellm::proj_w4_kernel<CB, NB, 2> : ellm::proj_w4_kernel<CB, NB, 1>;
+struct W4Choice {
+    W4Kernel kernel;
+    int threads, smem;
+};
+template <int CB, int WN, int NB>
+W4Choice w4_choice_of(size_t group) {
+    return {group == 128  ? ellm::proj_w4_kernel<CB, WN, NB, 4>
+            : group == 64 ? ellm::proj_w4_kernel<CB, WN, NB, 2>
+                          : ellm::proj_w4_kernel<CB, WN, NB, 1>,
+            ellm::W4Shape<CB, WN, NB>::kThreads, ellm::W4Shape<CB, WN, NB>::kSmemBytes};
 }
-// Column blocks per pass: as many as a CTA has (up to 4), so that a row fragment is fetched once for them.
-W4Kernel w4_kernel(int cb, int nb, size_t group) {
-    if (cb == 1) return nb == 1 ? w4_kernel_of<1, 1>(group) : w4_kernel_of<1, 2>(group);
-    if (cb == 2) return nb == 1 ? w4_kernel_of<2, 1>(group) : w4_kernel_of<2, 2>(group);
-    return nb == 1 ? w4_kernel_of<4, 1>(group) : w4_kernel_of<4, 2>(group);
-}
-int w4_column_blocks(size_t n, int sm_count) {
-    const size_t per_cta = ((n + 15) / 16 + sm_count - 1) / sm_count;
-    return per_cta >= 3 ? 4 : static_cast<int>(per_cta);
+// Warps across the columns and blocks per warp by the blocks a CTA has: one block leaves all 16 warps to K,
+// four and more put four warps across (a chunk of the rows then serves up to 16 blocks).
+template <int NB>
+W4Choice w4_choice(size_t n, size_t group, int sm_count) {
+    const size_t blocks = ((n + 15) / 16 + sm_count - 1) / sm_count;
+    if (blocks <= 1) return w4_choice_of<1, 1, NB>(group);
+    if (blocks <= 2) return w4_choice_of<1, 2, NB>(group);
+    if (blocks <= 4) return w4_choice_of<1, 4, NB>(group);
+    if (blocks <= 8) return w4_choice_of<2, 4, NB>(group);
+    return w4_choice_of<4, 4, NB>(group);
 }
 
 }  // namespace
@@ -554,9 +562,8 @@ int ellm_matmul_add_w4_create(const ellm_matmul_add_w4_desc* d, ellm_matmul_add_
     h->dw = *d;
     int st = proj_common_create(h, d->device, d->stream, d->async);
     if (st == ELLM_OK) {
-        const int cb = w4_column_blocks(d->n_max, h->plan.sm_count);
-        for (int nb = 1; nb <= 2 && st == ELLM_OK; ++nb)
-            if (cudaFuncSetAttribute(w4_kernel(cb, nb, d->group), cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::w4_smem_bytes(cb, nb)) != cudaSuccess)
+        for (const W4Choice& c : {w4_choice<1>(d->n_max, d->group, h->plan.sm_count), w4_choice<2>(d->n_max, d->group, h->plan.sm_count)})
+            if (cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, c.smem) != cudaSuccess)
                 st = fail(ELLM_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(cudaGetLastError()));
     }
     if (st == ELLM_OK && d->m_max > static_cast<size_t>(ellm::kW4MaxRows)) {
@@ -621,9 +628,9 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
         p.max_batch = static_cast<int>(d.max_batch);
         p.n_cols = static_cast<int>(d.n_max);
         p.k = static_cast<int>(d.k_max);
-        const int cb = w4_column_blocks(d.n_max, h->plan.sm_count), nb = rows > 8 ? 2 : 1;
+        const W4Choice c = rows > 8 ? w4_choice<2>(d.n_max, d.group, h->plan.sm_count) : w4_choice<1>(d.n_max, d.group, h->plan.sm_count);
         const unsigned grid = static_cast<unsigned>(std::min<size_t>((d.n_max + 15) / 16, static_cast<size_t>(h->plan.sm_count)));
-        ELLM_CUDA(launch_dependent(w4_kernel(cb, nb, d.group), grid, ellm::kW4Threads, static_cast<size_t>(ellm::w4_smem_bytes(cb, nb)), h->stream, p));
+        ELLM_CUDA(launch_dependent(c.kernel, grid, static_cast<unsigned>(c.threads), static_cast<size_t>(c.smem), h->stream, p));
         ++h->skinny_launches;
         return proj_finish(h);
     }
