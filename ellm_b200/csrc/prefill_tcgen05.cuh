@@ -103,6 +103,11 @@ struct Tcgen05Plan {
     CUtensorMap ext_q, ext_k, ext_v, ext_pk, ext_pv;
 };
 
+// kExt, capped scores: above kTcCapMax the polynomial's 7e-6 of a score of cap would pass a quarter of P's rounding
+// to bf16 (such chunks go to the warp-level kernel); up to kTcFixedMaxCap in log2 units the softmax takes 0 for the
+// row maximum: exp2 of +-88 and sums of 2^20 such are far from the ends of fp32's range.
+constexpr float kTcCapMax = 128.0f;
+constexpr float kTcFixedMaxCap = 88.0f;
 // kExt bits
 enum { kExtOn = 1, kExtCap = 2, kExtBias = 4, kExtSplit = 8 };
 
@@ -114,7 +119,7 @@ struct TcExt {
     int prefix_tiles = 0;           // 128-key tiles of the shared prefix
     int splits = 1;                 // kExtSplit: runs of prefix tiles, each with its own partial result
     long long part_rows = 0;        // kExtSplit: rows of one partial
-    float cap_coef[6] = {};         // the tanh polynomial times cap_log2
+    float cap_coef[5] = {};         // the tanh polynomial times cap_log2
     // q and the cache, for the rows recomputed key by key
     const __nv_bfloat16* q = nullptr;
     const __nv_bfloat16* k = nullptr;
@@ -286,6 +291,13 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* r) {
           "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -432,7 +444,6 @@ __device__ __forceinline__ int4 tc_range_of_positions(const TcParamsExt& p, int 
     const long long pre = p.ext.mods.prefix_lens ? p.ext.mods.prefix_lens[b] : 0;
     const long long ke = max(0ll, min(max(p1 + 1, pre), end));
     long long fhi = p0 < 0 ? 0 : min(max(p0 + 1, pre), end);
-    if (p.ext.mods.slopes) fhi = min(fhi, p0 + 1);   // beyond the position the distance changes sign
     return make_int4(0, static_cast<int>(ke), 0, static_cast<int>(max(0ll, fhi)));
 }
 
@@ -523,7 +534,6 @@ __global__ void __launch_bounds__(128) tc_ranges_kernel(const ScoreMods m, const
             atomicMax(&s[1], static_cast<int>(hi));
         }
         atomicMax(&s[2], static_cast<int>(lo));
-        if (m.slopes) hi = min(hi, pos + 1);
         atomicMin(&s[3], static_cast<int>(max(0ll, hi)));
     }
     __syncthreads();
@@ -535,28 +545,47 @@ struct TcRow {
     float scale_log2, cap_in, cap_log2;
     float slope;     // times log2(e)
     float dist0;     // position minus the tile's first key
+    bool ahead;      // no visible column lies beyond the row's position (uniform over the warp)
 };
-// One score in log2 units; column c of the tile.
+// One score in log2 units; column c of the tile.  The capped form here is 1 - 2 / (1 + e^(2u)) with an absolute
+// error of 1e-7 cap: the chunk kernel is used up to kTcCapMax.
 template <int kExt>
-__device__ __forceinline__ float tc_score(const TcRow& r, float t, int c) {
-    float x = (kExt & kExtCap) ? r.cap_log2 * tanh_any(t * r.cap_in) : t * r.scale_log2;
-    if (kExt & kExtBias) x -= r.slope * fabsf(r.dist0 - static_cast<float>(c));
+__device__ __forceinline__ float tc_score(const TcRow& r, float t, float c) {
+    float x = (kExt & kExtCap) ? fmaf(-2.0f * r.cap_log2, fast_rcp(1.0f + fast_exp2(t * (r.cap_in * 2.0f * kLog2e))), r.cap_log2)
+                               : t * r.scale_log2;
+    if (kExt & kExtBias) x = fmaf(-r.slope, fabsf(r.dist0 - c), x);
     return x;
 }
-// 64 products of one row (columns c0 ..) -> scores in log2 units plus `off`, in place.  kAhead: no column lies
-// beyond the row's position (the distance needs no absolute value).  All lanes of the warp call.
-template <int kExt, bool kAhead>
-__device__ __forceinline__ void tc_scores64(float (&s)[64], const TcRow& r, const float (&coef)[6], int c0, float off) {
-    // (opaque: 64 biases are cheaper computed again in the second pass than kept from the first)
-    float dist0 = r.dist0;
-    asm volatile("" : "+f"(dist0));
-    const float base = (kExt & kExtBias) && kAhead ? off - r.slope * (dist0 - static_cast<float>(c0)) : off;
-    const uint64_t base2 = pack2(base, base);
-    auto add_of = [&](int i) -> uint64_t {   // what is added to scores i, i + 1
-        if constexpr ((kExt & kExtBias) != 0 && kAhead) return pack2(fmaf(r.slope, static_cast<float>(i), base), fmaf(r.slope, static_cast<float>(i + 1), base));
-        else return base2;
-    };
-    bool poly = true;
+template <int kExt>
+__device__ __forceinline__ float tc_score_in(int col, float t, const TcRow& r, int lo, int rel) {
+    return col >= lo && col <= rel ? tc_score<kExt>(r, t, static_cast<float>(col)) : -INFINITY;
+}
+// 64 products of one row (columns c0 ..) -> scores in log2 units plus `off`, in place.  All lanes of the warp call.
+template <int kExt>
+__device__ __forceinline__ void tc_scores64(float (&s)[64], const TcRow& r, const float (&coef)[5], float c0, float off) {
+    if constexpr ((kExt & kExtBias) != 0) {
+        // the bias first, into `add`: with every column at or before the position it is linear in the column
+        const float d = r.dist0 - c0;
+        const float base = off - r.slope * d;
+        auto add_of = [&](int i) { return r.ahead ? fmaf(r.slope, static_cast<float>(i), base) : fmaf(-r.slope, fabsf(d - static_cast<float>(i)), off); };
+        if constexpr ((kExt & kExtCap) == 0) {
+            const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2);
+            if (r.ahead) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 2)
+                    unpack2(fma2(pack2(s[i], s[i + 1]), scale2, pack2(fmaf(r.slope, static_cast<float>(i), base), fmaf(r.slope, static_cast<float>(i + 1), base))), s[i], s[i + 1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] = fmaf(s[i], r.scale_log2, add_of(i));
+            }
+            return;
+        }
+    }
+    if constexpr ((kExt & kExtCap) == 0 && (kExt & kExtBias) == 0) {
+        const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2), off2 = pack2(off, off);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) unpack2(fma2(pack2(s[i], s[i + 1]), scale2, off2), s[i], s[i + 1]);
+    }
     if constexpr ((kExt & kExtCap) != 0) {
         float m0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), m1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
 #pragma unroll
@@ -565,42 +594,35 @@ __device__ __forceinline__ void tc_scores64(float (&s)[64], const TcRow& r, cons
             m1 = max3(m1, fabsf(s[i + 2]), fabsf(s[i + 3]));
         }
         m0 = max3(m0, fabsf(s[62]), fabsf(s[63]));
-        poly = __all_sync(0xffffffffu, fmaxf(m0, m1) * r.cap_in <= kTanhPolyMax);
-    }
-    if constexpr ((kExt & kExtCap) == 0) {
-        const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2);
+        const float o = (kExt & kExtBias) ? 0.0f : off;
+        if (__all_sync(0xffffffffu, fmaxf(m0, m1) * r.cap_in <= kTanhPolyMax)) {
+            const uint64_t in2 = pack2(r.cap_in, r.cap_in), o2 = pack2(o, o);
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) unpack2(fma2(pack2(s[i], s[i + 1]), scale2, add_of(i)), s[i], s[i + 1]);
-    } else if (poly) {
-        const uint64_t in2 = pack2(r.cap_in, r.cap_in);
-        uint64_t c[6];
+            for (int i = 0; i < 64; i += 2) {
+                const uint64_t u = mul2(pack2(s[i], s[i + 1]), in2), v = mul2(u, u);
+                uint64_t q = fma2(pack2(coef[4], coef[4]), v, pack2(coef[3], coef[3]));
+                q = fma2(q, v, pack2(coef[2], coef[2]));
+                q = fma2(q, v, pack2(coef[1], coef[1]));
+                q = fma2(q, v, pack2(coef[0], coef[0]));
+                unpack2(fma2(u, q, o2), s[i], s[i + 1]);
+            }
+        } else {
+            const float k = r.cap_in * (2.0f * kLog2e), top = r.cap_log2 + o, twice = -2.0f * r.cap_log2;
 #pragma unroll
-        for (int i = 0; i < 6; ++i) c[i] = pack2(coef[i], coef[i]);
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-            const uint64_t u = mul2(pack2(s[i], s[i + 1]), in2), v = mul2(u, u);
-            uint64_t q = fma2(c[5], v, c[4]);
-            q = fma2(q, v, c[3]);
-            q = fma2(q, v, c[2]);
-            q = fma2(q, v, c[1]);
-            q = fma2(q, v, c[0]);
-            unpack2(fma2(u, q, add_of(i)), s[i], s[i + 1]);
+            for (int i = 0; i < 64; ++i) s[i] = fmaf(twice, fast_rcp(1.0f + fast_exp2(s[i] * k)), top);
         }
-    } else {
+        if constexpr ((kExt & kExtBias) != 0) {
+            const float d = r.dist0 - c0, base = off - r.slope * d;
+            if (r.ahead) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-            float a0, a1;
-            unpack2(add_of(i), a0, a1);
-            s[i] = r.cap_log2 * tanh_any(s[i] * r.cap_in) + a0;
-            s[i + 1] = r.cap_log2 * tanh_any(s[i + 1] * r.cap_in) + a1;
+                for (int i = 0; i < 64; ++i) s[i] += fmaf(r.slope, static_cast<float>(i), base);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] += fmaf(-r.slope, fabsf(d - static_cast<float>(i)), off);
+            }
         }
-    }
-    if constexpr ((kExt & kExtBias) != 0 && !kAhead) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] -= r.slope * fabsf(dist0 - static_cast<float>(c0 + i));
     }
 }
-
 // A wait of the teardown: bounded, sets no status.
 __device__ __noinline__ bool mbar_wait_quiet(uint32_t bar, uint32_t parity, unsigned long long timeout_ns) {
     const unsigned long long t0 = global_timer_ns();
@@ -618,6 +640,8 @@ __device__ __noinline__ bool mbar_wait_quiet(uint32_t bar, uint32_t parity, unsi
 struct TcFixed {
     float m_used, l;
 };
+
+// kExt: ext = the row's constants and the visible columns.
 template <int kExt, class... Ext>
 __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, float scale_log2, float m_used, float l,
                                                    float first_half_sum, uint32_t* pk, const Ext... ext) {
@@ -629,7 +653,7 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         tmem_wait_ld();
         if constexpr (kExt != 0)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = tc_score<kExt>(ext..., v[i], 64 + c * 32 + i);
+            for (int i = 0; i < 32; ++i) v[i] = tc_score_in<kExt>(64 + c * 32 + i, v[i], ext...);
         float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
         for (int i = 6; i < 30; i += 6) {
@@ -642,8 +666,11 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
     }
     const float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * scale_log2);
     // rows whose maximum did not move far keep it (their corr is 1): as in the two-pass step
-    const bool moved = m_new - m_used > kTcRescaleThreshold;
-    const float corr = moved ? fast_exp2(m_used - m_new) : 1.0f;
+    bool moved = m_new - m_used > kTcRescaleThreshold;
+    if constexpr (kExt != 0) moved = moved && m_new != -INFINITY;
+    float corr = moved ? fast_exp2(m_used - m_new) : 1.0f;
+    if constexpr (kExt != 0)   // a row whose first key is in this half: nothing to bring along
+        if (moved && m_used == -INFINITY) corr = 0.0f;
     if (moved) m_used = m_new;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {   // O_t: every P.V of earlier steps has completed (this step's S_t exists)
@@ -665,7 +692,8 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         }
         tmem_st32u(tS, q);
     }
-    const uint64_t scale2 = pack2(scale_log2, scale_log2), negm2 = pack2(-m_used, -m_used);
+    const float msub = kExt != 0 && m_used == -INFINITY ? 0.0f : m_used;
+    const uint64_t scale2 = pack2(scale_log2, scale_log2), negm2 = pack2(-msub, -msub);
     uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
@@ -674,7 +702,7 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         tmem_wait_ld();
         if constexpr (kExt != 0)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = tc_score<kExt>(ext..., v[i], 64 + c * 32 + i);
+            for (int i = 0; i < 32; ++i) v[i] = tc_score_in<kExt>(64 + c * 32 + i, v[i], ext...);
 #pragma unroll
         for (int cc = 0; cc < 16; ++cc) {
             const uint64_t x2 = kExt != 0 ? add2(pack2(v[2 * cc], v[2 * cc + 1]), negm2) : fma2(pack2(v[2 * cc], v[2 * cc + 1]), scale2, negm2);
@@ -693,6 +721,121 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
     r.m_used = m_used;
     r.l = (l + first_half_sum) * corr + (sa + sb);
     return r;
+}
+
+// -infinity to the columns outside [lo, rel] (relative to the 64).
+__device__ __forceinline__ void tc_mask64(float (&s)[64], int lo, int rel) {
+    const unsigned long long below = rel < 0 ? 0ull : rel >= 63 ? ~0ull : (2ull << rel) - 1ull;
+    const unsigned long long from = lo <= 0 ? ~0ull : lo >= 64 ? 0ull : ~0ull << lo;
+    const unsigned m0 = static_cast<unsigned>(below & from), m1 = static_cast<unsigned>((below & from) >> 32);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[c] = (m0 >> c) & 1u ? s[c] : -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[32 + c] = (m1 >> c) & 1u ? s[32 + c] : -INFINITY;
+}
+
+// The two-pass step of a kExt row tile: the true maximum, O_t rescaled to it where it moved far, then P.  Taken for a
+// row tile's first key tile and when a score leaps far above the maximum in use.  32 columns at a time in a rolled
+// loop: it is rare, and its code must not push the one-pass step's out of the instruction cache.
+template <int kExt>
+__device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRow& r, int lo, int rel, bool rescale_o, float& m_used, float& l) {
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld32(tS + c * 32, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int col = c * 32 + i;
+            mx = fmaxf(mx, col >= lo && col <= rel ? tc_score<kExt>(r, v[i], static_cast<float>(col)) : -INFINITY);
+        }
+    }
+    const float m_new = fmaxf(m_used, mx);
+    const bool need = (m_new - m_used > kTcRescaleThreshold) || (m_used == -INFINITY && m_new != -INFINITY);
+    const bool rescale = __any_sync(0xffffffffu, need);
+    float corr = 1.0f;
+    if (rescale) {
+        corr = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
+        m_used = m_new;
+    }
+    const float msub = (m_used == -INFINITY) ? 0.0f : m_used;
+    if (rescale && rescale_o) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= corr;
+            tmem_st32(tO + c * 32, o);
+        }
+    }
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {   // P of 32 columns takes 16, which never overlap columns of S_t not yet read
+        float v[32];
+        uint32_t pk[16];
+        tmem_ld32(tS + c * 32, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int col = c * 32 + i;
+            v[i] = fast_exp2(col >= lo && col <= rel ? tc_score<kExt>(r, v[i], static_cast<float>(col)) - msub : -INFINITY);
+            sum += v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+        tmem_st16u(tS + c * 16, pk);
+    }
+    l = l * corr + sum;
+}
+
+// One key tile of a kExt row tile: P_t in tensor memory on return.  fixed_max: the scores are bounded (capped, no
+// bias), m_used is a constant for the whole row and nothing can leap.
+template <int kExt>
+__device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRow& r, const float (&coef)[5], int lo, int rel, bool edge,
+                                            bool first, bool fixed_max, bool valid, float& m_used, float& l) {
+    bool slow = first && !fixed_max;
+    if (!slow) {
+        float sum0 = 0.0f;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            float s[64];
+            tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
+            tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
+            tmem_wait_ld();
+            tc_scores64<kExt>(s, r, coef, static_cast<float>(half * 64), -m_used);
+            if (edge) tc_mask64(s, lo - half * 64, rel - half * 64);
+            uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                const float p0 = fast_exp2(s[2 * c]), p1 = fast_exp2(s[2 * c + 1]);
+                if (c & 1) sum_b = add2(sum_b, pack2(p0, p1)); else sum_a = add2(sum_a, pack2(p0, p1));
+                pk[c] = pack_bf16(p0, p1);
+            }
+            float sa, sb;
+            unpack2(add2(sum_a, sum_b), sa, sb);
+            const float sum = sa + sb;
+            // a row that saw no key before this tile has m_used = -infinity: its first one shows up here too
+            const bool leapt = !fixed_max && __any_sync(0xffffffffu, !(sum < kTcSumTrigger) && valid);
+            if (!leapt) {
+                tmem_st32u(tS + half * 32, pk);
+                if (half == 0) sum0 = sum; else l += sum0 + sum;
+            } else if (half == 0) {   // S_t is still intact: the whole step in two passes
+                slow = true;
+                break;
+            } else {                  // the first half's P is already in place: bring it and O_t to the new maximum
+                uint32_t redone[32];
+                const TcFixed f = tc_fix_second_half<kExt>(tS, tO, 0.0f, m_used, l, sum0, redone, r, edge ? lo : 0, edge ? rel : 127);
+                m_used = f.m_used;
+                l = f.l;
+                tmem_st32u(tS + 32, redone);
+            }
+        }
+    }
+    if (slow) tc_two_pass<kExt>(tS, tO, r, edge ? lo : 0, edge ? rel : 127, !first, m_used, l);
 }
 
 // kFused: the chunk's own K/V rows come from k_new / v_new and are written into the cache here (a
@@ -817,7 +960,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // kExt: the row's interval of own keys, its constants
             int row_lo = 0, row_hi = 0;
             TcRow xr{};
-            float coef[6] = {};
+            float coef[5] = {};
+            bool fixed_max = false;
             if constexpr (kExt != 0) {
                 if ((kExt & kExtSplit) == 0 && valid) {
                     long long a, z;
@@ -831,14 +975,16 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if ((kExt & kExtBias) && valid) xr.slope = p.ext.mods.slopes[it.kvh * p.group + g] * kLog2e;
                 if constexpr ((kExt & kExtCap) != 0)
 #pragma unroll
-                    for (int i = 0; i < 6; ++i) coef[i] = p.ext.cap_coef[i];
+                    for (int i = 0; i < 5; ++i) coef[i] = p.ext.cap_coef[i];
+                // capped scores lie in +-cap: with 2^(cap log2 e) far inside fp32's (and bf16's) range the softmax needs no maximum
+                fixed_max = (kExt & kExtCap) && !(kExt & kExtBias) && p.ext.mods.cap_log2 <= kTcFixedMaxCap;
             }
             const long long lim = valid ? min(it.base + pos, it.key_end - 1) : -1;   // last key this row may see
             const long long tile_min_lim = min(it.base + ((it.pair * kTcTiles + t) * kTcTileRows) / p.group, it.key_end - 1);
             const int my_steps = it.steps[t];
             long long row_index = (static_cast<long long>(pos) * p.max_batch + it.b) * p.q_heads + it.kvh * p.group + g;
             if constexpr ((kExt & kExtSplit) != 0) row_index += it.split * p.ext.part_rows;
-            float m_used = -INFINITY, l = 0.0f;
+            float m_used = kExt != 0 && fixed_max ? 0.0f : -INFINITY, l = 0.0f;
             for (int j = 0; j < my_steps && ok; ++j) {
                 // lane 0 polls the barrier, the warp follows (32 pollers per warp only add shared-memory traffic)
                 ok = lane == 0 ? mbar_wait(bar_s_full(t), (steps_done + j) & 1, abort_word, p.status, kTcWaitSFull, p.wait_timeout_ns) : true;
@@ -857,13 +1003,24 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         lo = 0;
                         rel = left < kTcKeys ? static_cast<int>(left) - 1 : kTcKeys - 1;
                         edge = left < kTcKeys;
+                        xr.ahead = true;
                     } else {
                         key0 = static_cast<long long>(it.j0 + j - it.np) * kTcKeys;
                         lo = min(max(row_lo - static_cast<int>(key0), 0), kTcKeys);
                         rel = min(max(row_hi - static_cast<int>(key0), 0), kTcKeys) - 1;
+                        xr.ahead = p.ext.mods.prefix_lens == nullptr ||
+                                   key0 + kTcKeys - 1 <= it.base + (it.pair * kTcTiles + t) * static_cast<long long>(p.ext.tile_pos);
                         edge = static_cast<int>(key0) < it.flo[t] || static_cast<int>(key0) + kTcKeys > it.fhi[t];
                     }
                     xr.dist0 = static_cast<float>(static_cast<int>(it.base + pos - key0));
+                }
+                if constexpr (kExt != 0) {
+                    tc_step_ext<kExt>(tS, tO, xr, coef, lo, rel, edge, j == 0, fixed_max, valid, m_used, l);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_p_full(t));
+                    continue;
                 }
                 // Fast path (every step but the first, unless a score leaps far above the maximum in use):
                 // exponentiate against the maximum already in use, in one pass.  P is held in registers
@@ -884,11 +1041,10 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                         tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                         tmem_wait_ld();
-                        if constexpr (kExt != 0) tc_scores64<kExt, true>(s, xr, coef, half * 64, -m_used);
                         uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll
                         for (int cc = 0; cc < 32; ++cc) {
-                            const uint64_t x2 = kExt != 0 ? pack2(s[2 * cc], s[2 * cc + 1]) : fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
+                            const uint64_t x2 = fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
                             uint64_t p2;
                             if (kTcPolyEvery > 0 && (cc % kTcPolyDiv) == kTcPolyDiv - 1) {
                                 p2 = exp2_poly2(x2);
@@ -907,7 +1063,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         half_sum[half] = sa + sb;
                         // No row maximum is tracked here.  A score far above the maximum in use shows up as a huge
                         // term of the sum (2^16 and more: one key 16 octaves above, or infinity).
-                        const bool leapt = __any_sync(0xffffffffu, !(half_sum[half] < kTcSumTrigger) && (kExt == 0 || valid));
+                        const bool leapt = __any_sync(0xffffffffu, !(half_sum[half] < kTcSumTrigger));
                         if (half == 0) {
                             if (leapt) {   // S_t is still intact: the whole step the slow way
                                 slow = true;
@@ -917,9 +1073,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         } else {
                             if (leapt) {   // the first half's P is already in place: bring it and O_t to the new maximum
                                 uint32_t redone[32];   // (addressable only here: pk itself stays in registers)
-                                TcFixed f;
-                                if constexpr (kExt != 0) f = tc_fix_second_half<kExt>(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone, xr);
-                                else f = tc_fix_second_half<0>(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone);
+                                const TcFixed f = tc_fix_second_half<0>(tS, tO, p.scale_log2, m_used, l, half_sum[0], redone);
                                 m_used = f.m_used;
                                 l = f.l;
 #pragma unroll
@@ -946,7 +1100,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         tmem_ld32(tS + h * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                         tmem_ld32(tS + h * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                         tmem_wait_ld();
-                        if constexpr (kExt != 0) tc_scores64<kExt, false>(s, xr, coef, h * 64, 0.0f);
                         if (edge) {
 #pragma unroll
                             for (int c = 0; c < 64; ++c) s[c] = (h * 64 + c <= rel && h * 64 + c >= lo) ? s[c] : -INFINITY;
@@ -964,7 +1117,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         m1 = max3(m1, s[62], s[63]);
                         mx = max3(mx, fmaxf(m0, m1), fmaxf(m2, m3));
                     }
-                    const float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * p.scale_log2);
+                    const float m_new = fmaxf(m_used, mx * p.scale_log2);
                     // rescale O only when the maximum moved far enough to matter; otherwise keep
                     // exponentiating against the stale maximum (O and l stay consistent with it)
                     const bool need = (m_new - m_used > kTcRescaleThreshold) || (m_used == -INFINITY && m_new != -INFINITY);
@@ -1001,7 +1154,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                             tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
                             tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
                             tmem_wait_ld();
-                            if constexpr (kExt != 0) tc_scores64<kExt, false>(s, xr, coef, half * 64, -msub);
                             if (edge) {
 #pragma unroll
                                 for (int c = 0; c < 64; ++c) s[c] = (half * 64 + c <= rel && half * 64 + c >= lo) ? s[c] : -INFINITY;
@@ -1010,7 +1162,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                             for (int cc = 0; cc < 32; ++cc) {
                                 const int c = half * 32 + cc;
-                                const uint64_t x2 = kExt != 0 ? pack2(s[2 * cc], s[2 * cc + 1]) : fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
+                                const uint64_t x2 = fma2(pack2(s[2 * cc], s[2 * cc + 1]), scale2, negm2);
                                 uint64_t p2;
                                 if (kTcPolyEvery > 0 && (c % kTcPolyDiv) == kTcPolyDiv - 1) {
                                     p2 = exp2_poly2(x2);
@@ -1739,8 +1891,8 @@ inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d
     p.ext.tile_pos = tile_pos;
     p.ext.tiles = static_cast<int>((interval + tile_pos - 1) / tile_pos);
     p.ext.prefix_tiles = static_cast<int>((mods.plen + kTcKeys - 1) / kTcKeys);
-    const float c[6] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4, kTanhC5};
-    for (int i = 0; i < 6; ++i) p.ext.cap_coef[i] = c[i] * mods.cap_log2;
+    const float c[5] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4};
+    for (int i = 0; i < 5; ++i) p.ext.cap_coef[i] = c[i] * mods.cap_log2;
     p.ext.q = static_cast<const __nv_bfloat16*>(d.q);
     p.ext.k = static_cast<const __nv_bfloat16*>(d.k_cache);
     p.ext.v = static_cast<const __nv_bfloat16*>(d.v_cache);
