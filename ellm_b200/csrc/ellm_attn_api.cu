@@ -477,7 +477,7 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
         else if (h->d.prefill_kernel == ELLM_PREFILL_AUTO) use_tc = ellm::tcgen05_prefers(h->tc, interval, h->group);
         if (ext)   // (a short chunk leaves most of a 128-row tile empty: the warp-level kernel, as above)
             use_tc = h->tc.ready_ext && h->d.prefill_kernel != ELLM_PREFILL_WARP_MMA &&
-                     h->mods.cap_log2 <= ellm::kTcCapMax * ellm::kLog2e &&
+                     ellm::tcgen05_takes_cap(h->mods) &&
                      (use_tc || interval * static_cast<size_t>(h->group) >= 16);
     }
     // the chunk's K/V rows go into the cache inside the attention kernel where that is possible (a decode

@@ -44,6 +44,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/ellm_attn.h"
@@ -106,7 +107,8 @@ struct Tcgen05Plan {
 // kExt, capped scores: above kTcCapMax the polynomial's 7e-6 of a score of cap would pass a quarter of P's rounding
 // to bf16 (such chunks go to the warp-level kernel); up to kTcFixedMaxCap in log2 units the softmax takes 0 for the
 // row maximum: exp2 of +-88 and sums of 2^20 such are far from the ends of fp32's range.
-constexpr float kTcCapMax = 128.0f;
+// (cap_in's 9th power is folded into a coefficient: it has to stay in fp32's range)
+constexpr float kTcCapMax = 128.0f, kTcCapInMin = 1.0f / 4096.0f, kTcCapInMax = 4096.0f;
 constexpr float kTcFixedMaxCap = 88.0f;
 // kExt bits
 enum { kExtOn = 1, kExtCap = 2, kExtBias = 4, kExtSplit = 8 };
@@ -119,7 +121,7 @@ struct TcExt {
     int prefix_tiles = 0;           // 128-key tiles of the shared prefix
     int splits = 1;                 // kExtSplit: runs of prefix tiles, each with its own partial result
     long long part_rows = 0;        // kExtSplit: rows of one partial
-    float cap_coef[5] = {};         // the tanh polynomial times cap_log2
+    float cap_coef[5] = {};         // the tanh polynomial in the product itself: coefficient of t^(2i+1), times cap_log2
     // q and the cache, for the rows recomputed key by key
     const __nv_bfloat16* q = nullptr;
     const __nv_bfloat16* k = nullptr;
@@ -385,6 +387,8 @@ struct TcItem {
 };
 // kExt: key tiles of the shared prefix (counted in steps), then own tiles from j0 on; row tile t sees the own
 // keys [flo, fhi) whole.
+// With a distance bias the own tiles are walked from the last to the first: the nearest keys, whose scores the bias
+// lowers least, set the maximum at once (from first to last a steep head's maximum leaps in every tile).
 struct TcItemExt : TcItem {
     int np;
     int p0 = 0, split = 0;   // kExtSplit: first prefix tile of the item's run
@@ -484,6 +488,10 @@ __device__ __forceinline__ void tc_item(const TcParamsExt& p, long long idx, TcI
             it.steps[t] = rows ? it.np + (r[t].x < r[t].y ? (r[t].y + kTcKeys - 1) / kTcKeys - it.j0 : 0) : 0;
             it.nsteps = max(it.nsteps, it.steps[t]);
         }
+        if (p.ext.mods.slopes)   // walked backwards: both row tiles start at the last tile (masked for the one it lies beyond)
+#pragma unroll
+            for (int t = 0; t < kTcTiles; ++t)
+                if (it.steps[t] > 0) it.steps[t] = it.nsteps;
         // as in tc_item, for the last own tile (a prefix tile is cut by its tensor map)
         it.zero_tail = p.positions != nullptr && it.nsteps > it.np &&
                        static_cast<long long>(it.j0 + it.nsteps - it.np) * kTcKeys > it.key_end;
@@ -559,69 +567,6 @@ __device__ __forceinline__ float tc_score(const TcRow& r, float t, float c) {
 template <int kExt>
 __device__ __forceinline__ float tc_score_in(int col, float t, const TcRow& r, int lo, int rel) {
     return col >= lo && col <= rel ? tc_score<kExt>(r, t, static_cast<float>(col)) : -INFINITY;
-}
-// 64 products of one row (columns c0 ..) -> scores in log2 units plus `off`, in place.  All lanes of the warp call.
-template <int kExt>
-__device__ __forceinline__ void tc_scores64(float (&s)[64], const TcRow& r, const float (&coef)[5], float c0, float off) {
-    if constexpr ((kExt & kExtBias) != 0) {
-        // the bias first, into `add`: with every column at or before the position it is linear in the column
-        const float d = r.dist0 - c0;
-        const float base = off - r.slope * d;
-        auto add_of = [&](int i) { return r.ahead ? fmaf(r.slope, static_cast<float>(i), base) : fmaf(-r.slope, fabsf(d - static_cast<float>(i)), off); };
-        if constexpr ((kExt & kExtCap) == 0) {
-            const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2);
-            if (r.ahead) {
-#pragma unroll
-                for (int i = 0; i < 64; i += 2)
-                    unpack2(fma2(pack2(s[i], s[i + 1]), scale2, pack2(fmaf(r.slope, static_cast<float>(i), base), fmaf(r.slope, static_cast<float>(i + 1), base))), s[i], s[i + 1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = fmaf(s[i], r.scale_log2, add_of(i));
-            }
-            return;
-        }
-    }
-    if constexpr ((kExt & kExtCap) == 0 && (kExt & kExtBias) == 0) {
-        const uint64_t scale2 = pack2(r.scale_log2, r.scale_log2), off2 = pack2(off, off);
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) unpack2(fma2(pack2(s[i], s[i + 1]), scale2, off2), s[i], s[i + 1]);
-    }
-    if constexpr ((kExt & kExtCap) != 0) {
-        float m0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), m1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
-#pragma unroll
-        for (int i = 6; i < 62; i += 4) {
-            m0 = max3(m0, fabsf(s[i]), fabsf(s[i + 1]));
-            m1 = max3(m1, fabsf(s[i + 2]), fabsf(s[i + 3]));
-        }
-        m0 = max3(m0, fabsf(s[62]), fabsf(s[63]));
-        const float o = (kExt & kExtBias) ? 0.0f : off;
-        if (__all_sync(0xffffffffu, fmaxf(m0, m1) * r.cap_in <= kTanhPolyMax)) {
-            const uint64_t in2 = pack2(r.cap_in, r.cap_in), o2 = pack2(o, o);
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-                const uint64_t u = mul2(pack2(s[i], s[i + 1]), in2), v = mul2(u, u);
-                uint64_t q = fma2(pack2(coef[4], coef[4]), v, pack2(coef[3], coef[3]));
-                q = fma2(q, v, pack2(coef[2], coef[2]));
-                q = fma2(q, v, pack2(coef[1], coef[1]));
-                q = fma2(q, v, pack2(coef[0], coef[0]));
-                unpack2(fma2(u, q, o2), s[i], s[i + 1]);
-            }
-        } else {
-            const float k = r.cap_in * (2.0f * kLog2e), top = r.cap_log2 + o, twice = -2.0f * r.cap_log2;
-#pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] = fmaf(twice, fast_rcp(1.0f + fast_exp2(s[i] * k)), top);
-        }
-        if constexpr ((kExt & kExtBias) != 0) {
-            const float d = r.dist0 - c0, base = off - r.slope * d;
-            if (r.ahead) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] += fmaf(r.slope, static_cast<float>(i), base);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] += fmaf(-r.slope, fabsf(d - static_cast<float>(i)), off);
-            }
-        }
-    }
 }
 // A wait of the teardown: bounded, sets no status.
 __device__ __noinline__ bool mbar_wait_quiet(uint32_t bar, uint32_t parity, unsigned long long timeout_ns) {
@@ -723,15 +668,79 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
     return r;
 }
 
-// -infinity to the columns outside [lo, rel] (relative to the 64).
-__device__ __forceinline__ void tc_mask64(float (&s)[64], int lo, int rel) {
-    const unsigned long long below = rel < 0 ? 0ull : rel >= 63 ? ~0ull : (2ull << rel) - 1ull;
-    const unsigned long long from = lo <= 0 ? ~0ull : lo >= 64 ? 0ull : ~0ull << lo;
-    const unsigned m0 = static_cast<unsigned>(below & from), m1 = static_cast<unsigned>((below & from) >> 32);
+// 64 products of one row -> P and its sum: score, subtraction of the maximum (inside `off`), mask, exp2, rounding,
+// pair by pair, so that the polynomial's multiply-adds and the exponentials are in flight together (computing all
+// scores first and all exponentials after ran the two units one after the other).
+//   kCap: the tanh polynomial with cap_in folded into its coefficients;  kScored: s holds scores already.
+//   m0, m1: visible columns;  base, slope: the distance bias of column i is base + slope * i (kExtBias, `ahead`).
+template <int kExt, bool kScored, bool kMask>
+__device__ __forceinline__ float tc_exp64(const float (&s)[64], const TcRow& r, const float (&coef)[5], float base, unsigned m0, unsigned m1,
+                                          uint32_t (&pk)[32]) {
+    const uint64_t base2 = pack2(base, base), scale2 = pack2(r.scale_log2, r.scale_log2);
+    uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
 #pragma unroll
-    for (int c = 0; c < 32; ++c) s[c] = (m0 >> c) & 1u ? s[c] : -INFINITY;
+    for (int c = 0; c < 32; ++c) {
+        const int i = 2 * c;
+        const uint64_t s2 = pack2(s[i], s[i + 1]);
+        uint64_t add = base2, x2;
+        if constexpr ((kExt & kExtBias) != 0 && !kScored) add = pack2(fmaf(r.slope, static_cast<float>(i), base), fmaf(r.slope, static_cast<float>(i + 1), base));
+        if constexpr (kScored) {
+            x2 = add2(s2, base2);
+        } else if constexpr ((kExt & kExtCap) != 0) {
+            const uint64_t v = mul2(s2, s2);
+            uint64_t q = fma2(pack2(coef[4], coef[4]), v, pack2(coef[3], coef[3]));
+            q = fma2(q, v, pack2(coef[2], coef[2]));
+            q = fma2(q, v, pack2(coef[1], coef[1]));
+            q = fma2(q, v, pack2(coef[0], coef[0]));
+            x2 = fma2(s2, q, add);
+        } else {
+            x2 = fma2(s2, scale2, add);
+        }
+        float x0, x1;
+        unpack2(x2, x0, x1);
+        if constexpr (kMask) {
+            const unsigned m = c < 16 ? m0 : m1;
+            x0 = (m >> (i & 31)) & 1u ? x0 : -INFINITY;
+            x1 = (m >> ((i + 1) & 31)) & 1u ? x1 : -INFINITY;
+        }
+        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+        if (c & 1) sum_b = add2(sum_b, pack2(p0, p1)); else sum_a = add2(sum_a, pack2(p0, p1));
+        pk[c] = pack_bf16(p0, p1);
+    }
+    float sa, sb;
+    unpack2(add2(sum_a, sum_b), sa, sb);
+    return sa + sb;
+}
+template <int kExt>
+__device__ __forceinline__ float tc_row64(float (&s)[64], const TcRow& r, const float (&coef)[5], float c0, float off, bool edge, int lo, int rel,
+                                          uint32_t (&pk)[32]) {
+    unsigned m0 = ~0u, m1 = ~0u;
+    if (edge) {
+        const unsigned long long below = rel < 0 ? 0ull : rel >= 63 ? ~0ull : (2ull << rel) - 1ull;
+        const unsigned long long from = lo <= 0 ? ~0ull : lo >= 64 ? 0ull : ~0ull << lo;
+        m0 = static_cast<unsigned>(below & from);
+        m1 = static_cast<unsigned>((below & from) >> 32);
+    }
+    const float d = r.dist0 - c0, base = (kExt & kExtBias) ? off - r.slope * d : off;
+    bool direct = true;
+    if constexpr ((kExt & kExtCap) != 0) {
+        float a0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), a1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
 #pragma unroll
-    for (int c = 0; c < 32; ++c) s[32 + c] = (m1 >> c) & 1u ? s[32 + c] : -INFINITY;
+        for (int i = 6; i < 62; i += 4) {
+            a0 = max3(a0, fabsf(s[i]), fabsf(s[i + 1]));
+            a1 = max3(a1, fabsf(s[i + 2]), fabsf(s[i + 3]));
+        }
+        a0 = max3(a0, fabsf(s[62]), fabsf(s[63]));
+        direct = __all_sync(0xffffffffu, fmaxf(a0, a1) * r.cap_in <= kTanhPolyMax);
+    }
+    if constexpr ((kExt & kExtBias) != 0) direct = direct && r.ahead;
+    if (direct) return edge ? tc_exp64<kExt, false, true>(s, r, coef, base, m0, m1, pk) : tc_exp64<kExt, false, false>(s, r, coef, base, m0, m1, pk);
+    if constexpr ((kExt & (kExtCap | kExtBias)) != 0) {   // scores past the polynomial's range, or keys past the position
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = tc_score<kExt>(r, s[i], c0 + static_cast<float>(i));
+        return tc_exp64<kExt, true, true>(s, r, coef, off, m0, m1, pk);
+    }
+    return 0.0f;
 }
 
 // The two-pass step of a kExt row tile: the true maximum, O_t rescaled to it where it moved far, then P.  Taken for a
@@ -805,19 +814,8 @@ __device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRo
             tmem_ld32(tS + half * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
             tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
             tmem_wait_ld();
-            tc_scores64<kExt>(s, r, coef, static_cast<float>(half * 64), -m_used);
-            if (edge) tc_mask64(s, lo - half * 64, rel - half * 64);
-            uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
             uint32_t pk[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                const float p0 = fast_exp2(s[2 * c]), p1 = fast_exp2(s[2 * c + 1]);
-                if (c & 1) sum_b = add2(sum_b, pack2(p0, p1)); else sum_a = add2(sum_a, pack2(p0, p1));
-                pk[c] = pack_bf16(p0, p1);
-            }
-            float sa, sb;
-            unpack2(add2(sum_a, sum_b), sa, sb);
-            const float sum = sa + sb;
+            const float sum = tc_row64<kExt>(s, r, coef, static_cast<float>(half * 64), -m_used, edge, lo - half * 64, rel - half * 64, pk);
             // a row that saw no key before this tile has m_used = -infinity: its first one shows up here too
             const bool leapt = !fixed_max && __any_sync(0xffffffffu, !(sum < kTcSumTrigger) && valid);
             if (!leapt) {
@@ -1005,7 +1003,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         edge = left < kTcKeys;
                         xr.ahead = true;
                     } else {
-                        key0 = static_cast<long long>(it.j0 + j - it.np) * kTcKeys;
+                        key0 = static_cast<long long>((kExt & kExtBias) ? it.j0 + it.nsteps - 1 - j : it.j0 + j - it.np) * kTcKeys;
                         lo = min(max(row_lo - static_cast<int>(key0), 0), kTcKeys);
                         rel = min(max(row_hi - static_cast<int>(key0), 0), kTcKeys) - 1;
                         xr.ahead = p.ext.mods.prefix_lens == nullptr ||
@@ -1365,16 +1363,29 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                 row0 = (it.p0 + (item >> 1)) * kTcKeys;
                                 seq = 0;
                             } else {
-                                row0 -= it.np * kTcKeys;
+                                row0 = (kExt & kExtBias) ? (it.j0 + it.nsteps - 1 - (item >> 1)) * kTcKeys : row0 - it.np * kTcKeys;
                             }
                         }
                         mbar_arrive_expect_tx(bar_kv_full(slot), kTcTileBytes);
                         for (int h = 0; h < 2; ++h)
                             tma_load_4d(smem_base + kTcSmemRing + slot * kTcTileBytes + h * kTcHalfBytes, map, bar_kv_full(slot),
                                         h * 64, row0, it.kvh, seq);
+                        if constexpr ((kExt & kExtBias) != 0)
+                            if (it.zero_tail && item == 1) {   // walked backwards: the tile to clean up is the first V tile
+                                ok = mbar_wait(bar_kv_full(slot), round_par, abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
+                                if (!ok) break;
+                                const int first = static_cast<int>(it.key_end - static_cast<long long>(row0));
+                                unsigned char* tile = smem + kTcSmemRing + slot * kTcTileBytes;
+                                for (int r = first * 8; r < kTcKeys * 8; ++r) {
+                                    *reinterpret_cast<uint4*>(tile + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                    *reinterpret_cast<uint4*>(tile + kTcHalfBytes + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                }
+                                fence_async_smem();
+                                mbar_arrive(bar_tail);
+                            }
                     }
                 }
-                if (ok && it.zero_tail && it.nsteps > 0) {
+                if ((kExt & kExtBias) == 0 && ok && it.zero_tail && it.nsteps > 0) {
                     const long long last = ring_n - 1;   // the last V tile
                     const int slot = static_cast<int>(last % kTcStages);
                     ok = mbar_wait(bar_kv_full(slot), static_cast<uint32_t>((last / kTcStages) & 1), abort_word, p.status, kTcWaitKvFull,
@@ -1459,7 +1470,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // ring item i of this work item: K_(i/2) for even i, V_(i/2) for odd i
                 auto wait_item = [&](int item) {
                     const long long r = ring_c + item;
-                    if (it.zero_tail && item == 2 * nsteps - 1)   // the last V tile is released by the producer's clean-up
+                    if (it.zero_tail && item == ((kExt & kExtBias) ? 1 : 2 * nsteps - 1))   // this V tile is released by the producer's clean-up
                         return mbar_wait(bar_tail, static_cast<uint32_t>(tails & 1), abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
                     return mbar_wait(bar_kv_full(static_cast<int>(r % kTcStages)), static_cast<uint32_t>((r / kTcStages) & 1), abort_word,
                                      p.status, kTcWaitKvFull, p.wait_timeout_ns);
@@ -1826,6 +1837,10 @@ inline int launch_prefix_split(Tcgen05Plan& plan, const ellm_attn_desc& d, const
     return e == cudaSuccess ? ELLM_OK : ELLM_ERR_CUDA;
 }
 
+inline bool tcgen05_takes_cap(const ScoreMods& m) {
+    return m.cap_log2 == 0.0f || (m.cap_log2 <= kTcCapMax * kLog2e && m.cap_in >= kTcCapInMin && m.cap_in <= kTcCapInMax);
+}
+
 // A chunk with modified scores, row intervals or a shared prefix (bf16 result).
 inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d, const ScoreMods& mods, const int32_t* positions,
                                       size_t position_index, size_t interval, size_t batch, float* lse, int* status,
@@ -1892,7 +1907,7 @@ inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d
     p.ext.tiles = static_cast<int>((interval + tile_pos - 1) / tile_pos);
     p.ext.prefix_tiles = static_cast<int>((mods.plen + kTcKeys - 1) / kTcKeys);
     const float c[5] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4};
-    for (int i = 0; i < 5; ++i) p.ext.cap_coef[i] = c[i] * mods.cap_log2;
+    for (int i = 0; i < 5; ++i) p.ext.cap_coef[i] = static_cast<float>(c[i] * std::pow(static_cast<double>(mods.cap_in), 2 * i + 1) * mods.cap_log2);
     p.ext.q = static_cast<const __nv_bfloat16*>(d.q);
     p.ext.k = static_cast<const __nv_bfloat16*>(d.k_cache);
     p.ext.v = static_cast<const __nv_bfloat16*>(d.v_cache);
