@@ -271,9 +271,12 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
     const int pieces_cap = std::min(p.num_ctas + (kind == ellm::kMergePrefix ? p.pre_parts : 0), ellm::kMergeMaxPieces);
     const size_t smem = ellm::merge_smem_bytes(static_cast<int>(batch), pieces_cap);
     const bool light = blocks >= 128;
+    // with a shared prefix every row has one more piece per run of prefix tiles, 20 to 40 in all: all of them in
+    // flight at once, by four warps, or by two when the rows alone fill the SMs
+    const bool few = blocks < 1024;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(light ? ellm::kMergeLightThreads : ellm::kMergeThreads);
+    cfg.blockDim = dim3(kind == ellm::kMergePrefix ? (few ? 128 : 64) : light ? ellm::kMergeLightThreads : ellm::kMergeThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -286,8 +289,8 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
         return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, ellm::kMergeMods>, p, ob, lse_out, pieces_cap)
                      : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, ellm::kMergeMods>, p, ob, lse_out, pieces_cap);
     if (kind == ellm::kMergePrefix)
-        return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap)
-                     : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap);
+        return few ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 4, 8, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap)
+                   : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 10, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap);
     if (out_f32)
         return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 2, 4>, p, out_f32, lse_out, pieces_cap)
                      : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 8, 10>, p, out_f32, lse_out, pieces_cap);

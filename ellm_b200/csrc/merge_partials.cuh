@@ -56,7 +56,7 @@ template <typename OutT, int kWarps, int kAhead, int kKind = kMergePlain>
 // (both shapes are held to 64 registers: they have to fit beside two decode CTAs of ~184 registers x 128 threads -
 // one wide CTA, or the light shape's three or four per SM - or they cannot move in, and release their own
 // dependents, before the decode grid has drained)
-__global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : 20) decode_merge_kernel(const DecodeParams p, OutT* out, float* lse, int pieces_cap) {
+__global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : kWarps == 4 ? 8 : kAhead > 4 ? 14 : 20) decode_merge_kernel(const DecodeParams p, OutT* out, float* lse, int pieces_cap) {
     // a following kernel launched as a programmatic dependent may start its own prologue now
     ChainTrace ct(3);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
