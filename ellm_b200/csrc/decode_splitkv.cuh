@@ -71,12 +71,15 @@ struct DecodeParams {
     // Only what that kernel cannot have written is touched early: the positions, and cache rows
     // below each sequence's newest row; the queries and the stages that hold a newest row wait.
     int early = 0;
+    // kDecPrefix: the shared prefix (mods.pk, mods.pv, mods.plen) as further segments of the tile list
+    int pre_tiles = 0;             // 64-key tiles of the prefix
+    int pre_blocks = 0;            // blocks of 16 query rows per KV head = ceil(batch * group / 16)
     // The shared-prefix part of the step, for the merge: pre_parts partials [pre_rows, 128] and [pre_rows]
     const float* pre_o = nullptr;
     const float* pre_lse = nullptr;
     long long pre_rows = 0;
     int pre_parts = 0;
-    // kMods instantiations: capped / biased scores, keys from row_begin[b][position] on (key_begin is 0)
+    // kDecMods: capped / biased scores, keys from row_begin[b][position] on (key_begin is 0)
     ScoreMods mods;
 };
 
@@ -104,6 +107,12 @@ __device__ __forceinline__ int dec_tiles_of(long long begin, long long len) {
 // again: they may live in page-locked host memory).  All threads call.  The positions are fetched by as many threads as there are
 // sequences (one global-memory latency, not one per sequence); the running sum over the
 // per-sequence tile counts is then a short loop over shared memory.
+// What a decode step has beyond plain attention.  kDecMods: scores capped and biased, first keys per sequence.
+// kDecPrefix: a shared prefix, as segments (KV head, block of 16 of the step's query rows) behind the sequences' own
+// in the same tile list - the prefix is read once per 16 query rows, mostly from L2, by the one launch there
+// is anyway.  (Steps with more work take the tensor-memory kernel for the prefix, see launch_decode.)
+enum { kDecPlain = 0, kDecMods = 1, kDecPrefix = 2 };
+
 // kMods: the keys start at row_begin[b][position]; begs[b] receives that (where begs is given).
 template <bool kMods = false>
 __device__ inline void dec_build_prefix(const DecodeParams& p, int* prefix, int* lens, int* begs = nullptr) {
@@ -209,8 +218,9 @@ struct ModScore {
     }
 };
 
-template <int NB, bool kMods = false>
+template <int NB, int kKind = kDecPlain>
 __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const DecodeParams p) {
+    constexpr bool kMods = kKind == kDecMods;
     extern __shared__ __align__(128) unsigned char smem[];
     int* prefix = reinterpret_cast<int*>(smem + kDecWarps * kDecStages * kDecWarpStageBytes);   // [kDecMaxBatch + 1]
     int* lens = prefix + kDecMaxBatch + 1;                                                        // [kDecMaxBatch]
@@ -232,9 +242,10 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
     }
     dec_build_prefix<kMods>(p, prefix, lens, begs);
     const long long segs_per_seq = static_cast<long long>(p.kv_heads) * p.gtiles;
-    const long long total = static_cast<long long>(prefix[p.batch]) * segs_per_seq;
+    const long long own_total = static_cast<long long>(prefix[p.batch]) * segs_per_seq;
+    const long long total = kKind == kDecPrefix ? own_total + static_cast<long long>(p.kv_heads) * p.pre_blocks * p.pre_tiles : own_total;
     long long t_begin = 0, t_end = 0;
-    const bool has_tiles = dec_split_is_aligned(p, prefix, segs_per_seq, total)
+    const bool has_tiles = kKind != kDecPrefix && dec_split_is_aligned(p, prefix, segs_per_seq, total)
                                ? dec_aligned_range(p, prefix, segs_per_seq, total, blockIdx.x, &t_begin, &t_end)
                                : assign_range(total, p.num_ctas, blockIdx.x, &t_begin, &t_end);
     if (!has_tiles) {
@@ -245,27 +256,30 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
     long long t = t_begin;
     while (t < t_end) {
         // ---- locate the piece: segment of tile t and how far it runs ----
-        const int b = dec_find_seq(prefix, p.batch, segs_per_seq, t);
-        const int tiles_b = prefix[b + 1] - prefix[b];
-        const long long seq_base = static_cast<long long>(prefix[b]) * segs_per_seq;
+        const bool pre = kKind == kDecPrefix && t >= own_total;   // a piece of the shared prefix
+        const int b = pre ? 0 : dec_find_seq(prefix, p.batch, segs_per_seq, t);
+        const int tiles_b = pre ? p.pre_tiles : prefix[b + 1] - prefix[b];
+        const long long seq_base = pre ? own_total : static_cast<long long>(prefix[b]) * segs_per_seq;
         const int seg_in_seq = static_cast<int>((t - seq_base) / tiles_b);
         const int tile0 = static_cast<int>((t - seq_base) % tiles_b);
         const long long seg_end = seq_base + static_cast<long long>(seg_in_seq + 1) * tiles_b;
         const long long piece_end = seg_end < t_end ? seg_end : t_end;
         const int ntiles = static_cast<int>(piece_end - t);
-        const int kvh = seg_in_seq / p.gtiles, gt = seg_in_seq % p.gtiles;
-        const long long segment = static_cast<long long>(b) * segs_per_seq + seg_in_seq;
-        const long long len_raw = lens[b];
-        const long long len = len_raw < p.len_cap ? len_raw : p.len_cap;
-        const int rows_valid = min(16, p.group - gt * 16);
+        const int per_head = pre ? p.pre_blocks : p.gtiles;
+        const int kvh = seg_in_seq / per_head, gt = seg_in_seq % per_head;
+        const long long segment = (pre ? static_cast<long long>(p.batch) : static_cast<long long>(b)) * segs_per_seq + seg_in_seq;
+        const long long len_raw = pre ? p.mods.plen : lens[b];
+        const long long len = pre ? p.mods.plen : len_raw < p.len_cap ? len_raw : p.len_cap;
+        const int rows_valid = min(16, (pre ? p.batch * p.group : p.group) - gt * 16);
         const long long key0 = (kMods ? static_cast<long long>(begs[b]) : p.key_begin) + static_cast<long long>(tile0) * kDecTileKeys + warp * 16;
-        const __nv_bfloat16* kbase = p.k_cache + b * p.s0 + kvh * p.s1;
-        const __nv_bfloat16* vbase = p.v_cache + b * p.s0 + kvh * p.s1;
+        const __nv_bfloat16* kbase = pre ? p.mods.pk + kvh * p.mods.ps1 : p.k_cache + b * p.s0 + kvh * p.s1;
+        const __nv_bfloat16* vbase = pre ? p.mods.pv + kvh * p.mods.ps1 : p.v_cache + b * p.s0 + kvh * p.s1;
+        const long long s2 = pre ? p.mods.ps2 : p.s2;
         // fused append: position of the new token's row and where its K/V come from
         // the row being appended is the sequence's last key, unless its position lies past the
         // cache (then len was capped and nothing is read or written there)
         long long new_pos = -1;
-        if (p.k_new && len_raw == len) new_pos = len - 1;
+        if (p.k_new && len_raw == len && !pre) new_pos = len - 1;
         const __nv_bfloat16* knew = p.k_new ? p.k_new + (static_cast<long long>(b) * p.kv_heads + kvh) * kHeadDim : nullptr;
         const __nv_bfloat16* vnew = p.k_new ? p.v_new + (static_cast<long long>(b) * p.kv_heads + kvh) * kHeadDim : nullptr;
 
@@ -283,7 +297,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
                     const int row = (lane >> 4) + 2 * i;
                     const long long key = kfirst + row;
                     const bool ok = key < len;
-                    const long long off = (ok ? key : 0) * p.s2 + chunk * 8;
+                    const long long off = (ok ? key : 0) * s2 + chunk * 8;
                     cp_async_16(sK + swz_off(row, chunk), kbase + off, ok ? 16 : 0);
                     cp_async_16(sV + swz_off(row, chunk), vbase + off, ok ? 16 : 0);
                 }
@@ -293,7 +307,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
                     const int row = (lane >> 4) + 2 * i;
                     const long long key = kfirst + row;
                     const bool ok = key < len;
-                    const long long off = (ok ? key : 0) * p.s2 + chunk * 8;
+                    const long long off = (ok ? key : 0) * s2 + chunk * 8;
                     if (key == new_pos) {   // stream the new row from k_new / v_new ...
                         cp_async_16(sK + swz_off(row, chunk), knew + chunk * 8, 16);
                         cp_async_16(sV + swz_off(row, chunk), vnew + chunk * 8, 16);
@@ -346,8 +360,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
         for (int nb = 0; nb < NB; ++nb) {
             const int head = nb * 8 + (lane >> 2);
             const bool hv = head < rows_valid;
-            const __nv_bfloat16* qrow =
-                p.q + (static_cast<long long>(b) * p.q_heads + kvh * p.group + gt * 16 + (hv ? head : 0)) * kHeadDim + (lane & 3) * 2;
+            long long row = static_cast<long long>(b) * p.q_heads + kvh * p.group + gt * 16 + (hv ? head : 0);
+            if (pre) {   // query rows of the step, all sequences' heads of this KV head one after the other
+                const int rho = gt * 16 + (hv ? head : 0);
+                row = static_cast<long long>(rho / p.group) * p.q_heads + kvh * p.group + rho % p.group;
+            }
+            const __nv_bfloat16* qrow = p.q + row * kHeadDim + (lane & 3) * 2;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
                 qb[nb][ks][0] = hv ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16) : 0u;

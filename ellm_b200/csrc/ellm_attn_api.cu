@@ -163,6 +163,7 @@ struct ellm_attn {
     bool scores_on = false, prefix_on = false;
     float* pre_part = nullptr;         // shared prefix, decode steps: partial O [pre_slots][128], then partial LSE [pre_slots]
     size_t pre_slots = 0;
+    double prefix_flat_flops = 1.2e9;  // see prefix_is_flat
     std::mutex mu;
     uint64_t launches[ELLM_KERNEL_COUNT] = {};
     uint64_t timed[ELLM_KERNEL_COUNT] = {};
@@ -274,9 +275,10 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
     // with a shared prefix every row has one more piece per run of prefix tiles, 20 to 40 in all: all of them in
     // flight at once, by four warps, or by two when the rows alone fill the SMs
     const bool few = blocks < 1024;
+    const bool with_prefix = kind == ellm::kMergePrefix || kind == ellm::kMergePrefixFlat;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kind == ellm::kMergePrefix ? (few ? 128 : 64) : light ? ellm::kMergeLightThreads : ellm::kMergeThreads);
+    cfg.blockDim = dim3(with_prefix ? (few ? 128 : 64) : light ? ellm::kMergeLightThreads : ellm::kMergeThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -291,11 +293,24 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
     if (kind == ellm::kMergePrefix)
         return few ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 4, 8, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap)
                    : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 10, ellm::kMergePrefix>, p, ob, lse_out, pieces_cap);
+    if (kind == ellm::kMergePrefixFlat)
+        return few ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 4, 8, ellm::kMergePrefixFlat>, p, ob, lse_out, pieces_cap)
+                   : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 10, ellm::kMergePrefixFlat>, p, ob, lse_out, pieces_cap);
     if (out_f32)
         return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 2, 4>, p, out_f32, lse_out, pieces_cap)
                      : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<float, 8, 10>, p, out_f32, lse_out, pieces_cap);
     return light ? cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 2, 4>, p, ob, lse_out, pieces_cap)
                  : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10>, p, ob, lse_out, pieces_cap);
+}
+
+// Whether a decode step takes its shared prefix in the split-KV kernel's own tile list (one launch less, the
+// prefix read once per 16 query rows, warp-level products) or in the tensor-memory kernel (once per 256 rows, a
+// launch and a start-up of about 12 us more).  By the prefix's FLOPs.
+bool prefix_is_flat(const ellm_attn* h, size_t batch) {
+    return !h->tc.ready_ext || 4.0 * ellm::kHeadDim * static_cast<double>(h->mods.plen) * static_cast<double>(batch * h->d.q_heads) < h->prefix_flat_flops;
+}
+size_t prefix_flat_slots(const ellm_attn* h) {
+    return h->slots + h->d.kv_heads * ((h->d.max_batch * h->group + 15) / 16);
 }
 
 // Decode (interval == 1): K2 then K3.  out_f32 != nullptr selects the fp32
@@ -328,8 +343,16 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
     p.scale_log2 = h->d.scale * ellm::kLog2e;
     p.num_ctas = h->dec_ctas;
     p.mods = h->mods;
-    if (h->prefix_on) {
+    int merge_kind = h->scores_on ? ellm::kMergeMods : ellm::kMergePlain;
+    if (h->prefix_on && prefix_is_flat(h, batch)) {
+        merge_kind = ellm::kMergePrefixFlat;
+        p.pre_tiles = static_cast<int>((h->mods.plen + ellm::kDecTileKeys - 1) / ellm::kDecTileKeys);
+        p.pre_blocks = static_cast<int>((batch * h->group + 15) / 16);
+        p.part_o = h->pre_part;
+        p.part_lse = h->pre_part + h->pre_slots * ellm::kHeadDim;
+    } else if (h->prefix_on) {
         // the prefix's part first; the own keys' kernel and the merge follow
+        merge_kind = ellm::kMergePrefix;
         const int splits = ellm::prefix_splits(h->tc, batch, h->d.q_heads, h->d.kv_heads, (h->mods.plen + ellm::kTcKeys - 1) / ellm::kTcKeys);
         p.pre_rows = static_cast<long long>(batch * h->d.q_heads);
         p.pre_parts = splits;
@@ -351,10 +374,12 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
         LaunchScope ls(h, ELLM_KERNEL_DECODE_SPLITKV);
         if (h->scores_on) {
             if (h->group <= 8)
-                launch_dependent(ellm::decode_splitkv_kernel<1, true>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
+                launch_dependent(ellm::decode_splitkv_kernel<1, ellm::kDecMods>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
             else
-                launch_dependent(ellm::decode_splitkv_kernel<2, true>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
-        } else if (h->group <= 8)   // blocks of 8 query heads per segment: one for groups of up to 8 heads, else two
+                launch_dependent(ellm::decode_splitkv_kernel<2, ellm::kDecMods>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
+        } else if (merge_kind == ellm::kMergePrefixFlat)
+            launch_dependent(ellm::decode_splitkv_kernel<2, ellm::kDecPrefix>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
+        else if (h->group <= 8)   // blocks of 8 query heads per segment: one for groups of up to 8 heads, else two
             launch_dependent(ellm::decode_splitkv_kernel<1>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
         else
             launch_dependent(ellm::decode_splitkv_kernel<2>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
@@ -366,8 +391,7 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
         // its first instruction waits for the decode grid's memory to be visible
         LaunchScope ls(h, ELLM_KERNEL_MERGE);
         const cudaError_t e = launch_merge(p, batch, blocks, out_f32, out_f32 ? nullptr : (out_override ? out_override : h->d.out),
-                                           lse_out, h->stream, true,
-                                           h->prefix_on ? ellm::kMergePrefix : h->scores_on ? ellm::kMergeMods : ellm::kMergePlain);
+                                           lse_out, h->stream, true, merge_kind);
         if (e != cudaSuccess) return fail(ELLM_ERR_CUDA, "merge launch failed: %s", cudaGetErrorString(e));
     }
     ELLM_CUDA(cudaGetLastError());
@@ -376,12 +400,12 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
 
 int launch_prefill_warp_mma(ellm_attn* h, const int32_t* positions, size_t position_index,
                             size_t interval, size_t batch, long long key_begin, long long key_end,
-                            float* out_f32, float* lse_out, void* out_override = nullptr) {
+                            float* out_f32, float* lse_out) {
     ellm::PrefillParams p;
     p.q = static_cast<const __nv_bfloat16*>(h->d.q);
     p.k_cache = static_cast<const __nv_bfloat16*>(h->d.k_cache);
     p.v_cache = static_cast<const __nv_bfloat16*>(h->d.v_cache);
-    p.out = out_f32 ? static_cast<void*>(out_f32) : (out_override ? out_override : h->d.out);
+    p.out = out_f32 ? static_cast<void*>(out_f32) : h->d.out;
     p.lse = lse_out;
     p.positions = positions;
     p.position_index = static_cast<long long>(position_index);
@@ -489,16 +513,13 @@ int run_impl(ellm_attn* h, const int32_t* positions, size_t position_index, size
     const bool fused = use_tc && do_append && !out_f32 && !ext &&
                        ellm::tcgen05_can_fuse_append(h->tc, h->d, positions, position_index, batch, key_begin, key_end);
     // (a decode step whose rows may see nothing would not visit the newest row: appended up front as well)
-    const bool prefix_warp = h->prefix_on && !h->tc.ready_ext;   // more than 128 query heads per KV head
-    const bool decode_appends = !prefix_warp && !h->mods.row_begin;
+    const bool decode_appends = !h->mods.row_begin;
     if (do_append && (interval > 1 || !decode_appends) && !fused) {
         rc = launch_append(h, h->stream, h->d.k_cache, h->d.v_cache, h->d.k_new, h->d.v_new, h->d.kv_strides,
                            h->d.max_batch, h->d.kv_heads, h->d.max_seq, position_index, positions, interval, batch);
         if (rc) return rc;
     }
-    if (interval == 1 && prefix_warp) {
-        rc = launch_prefill_warp_mma(h, positions, position_index, interval, batch, key_begin, key_end, nullptr, lse_out, decode_out_override);
-    } else if (interval == 1) {
+    if (interval == 1) {
         // early streaming only where the caller vouched for it, and never for a step whose inputs the
         // library itself stages right before (the host-buffer entry point passes a stream override)
         rc = launch_decode(h, positions, position_index, batch, key_begin, key_end, out_f32, lse_out, do_append && decode_appends,
@@ -586,8 +607,9 @@ int ellm_attn_create(const ellm_attn_desc* desc, ellm_attn** out) {
     if (cudaMemset(h->status_dev, 0, 4 * sizeof(int)) != cudaSuccess) return cleanup(fail(ELLM_ERR_CUDA, "memset failed"));
     if (cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
-        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
-        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, ellm::kDecPrefix>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1, ellm::kDecMods>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, ellm::kDecMods>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<__nv_bfloat16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess)
@@ -1261,9 +1283,11 @@ int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size
     m.ps1 = static_cast<long long>(kv_head_stride);
     m.ps2 = static_cast<long long>(position_stride);
     m.plen = static_cast<long long>(prefix_len);
-    if (!h->pre_part && h->tc.ready_ext) {   // one partial row per (run of prefix tiles, query row), for any batch and prefix length
-        size_t slots = 0;
-        for (size_t b = 1; b <= h->d.max_batch; ++b)
+    if (!h->pre_part) {
+        // partial rows, for any batch and prefix length: 16 per slot of the split-KV kernel with the prefix in its
+        // tile list, or one per (run of prefix tiles, query row) of the tensor-memory kernel
+        size_t slots = prefix_flat_slots(h) * 16;
+        for (size_t b = 1; b <= h->d.max_batch && h->tc.ready_ext; ++b)
             slots = std::max(slots, b * h->d.q_heads * ellm::prefix_splits(h->tc, b, h->d.q_heads, h->d.kv_heads, INT64_MAX));
         DeviceGuard guard(h->d.device);
         if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", h->d.device);
@@ -1295,6 +1319,11 @@ int ellm_attn_set_option(ellm_attn* h, const char* name, long long value) {
     }
     if (std::strcmp(name, "decode_early_stream") == 0) {
         h->decode_early = value != 0;
+        return ELLM_OK;
+    }
+    if (std::strcmp(name, "prefix_flat_mflops") == 0) {
+        if (value < 0) return fail(ELLM_ERR_INVALID_ARG, "prefix_flat_mflops must be >= 0");
+        h->prefix_flat_flops = static_cast<double>(value) * 1e6;
         return ELLM_OK;
     }
     if (std::strcmp(name, "tc_fuse_append") == 0) {

@@ -50,8 +50,9 @@ __host__ __device__ inline size_t merge_smem_bytes(int batch, int pieces_cap) {
 }
 
 // kKind: kMergePlain, kMergeMods (the sequences' keys start at row_begin), kMergePrefix (the step has a shared
-// prefix, whose partials - one per run of prefix tiles, of all rows - are further pieces of every row).
-enum { kMergePlain = 0, kMergeMods = 1, kMergePrefix = 2 };
+// prefix, whose partials - one per run of prefix tiles, of all rows - are further pieces of every row),
+// kMergePrefixFlat (the prefix was part of the decode kernel's tile list: its pieces lie in the same workspace).
+enum { kMergePlain = 0, kMergeMods = 1, kMergePrefix = 2, kMergePrefixFlat = 3 };
 template <typename OutT, int kWarps, int kAhead, int kKind = kMergePlain>
 // (both shapes are held to 64 registers: they have to fit beside two decode CTAs of ~184 registers x 128 threads -
 // one wide CTA, or the light shape's three or four per SM - or they cannot move in, and release their own
@@ -79,12 +80,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : kWarps == 4 ? 8
     const int seg_in_seq = kvh * p.gtiles + gt;
     const long long segment = b * segs_per_seq + seg_in_seq;
     const int tiles_b = s_prefix[b + 1] - s_prefix[b];
-    const long long total = static_cast<long long>(s_prefix[p.batch]) * segs_per_seq;
+    const long long own_total = static_cast<long long>(s_prefix[p.batch]) * segs_per_seq;
+    const long long total = kKind == kMergePrefixFlat ? own_total + static_cast<long long>(p.kv_heads) * p.pre_blocks * p.pre_tiles : own_total;
     OutT* orow = out + row * kHeadDim + lane * 4;
     long long c_first = 0, c_last = -1;
     if (tiles_b > 0) {
         const long long t0 = static_cast<long long>(s_prefix[b]) * segs_per_seq + static_cast<long long>(seg_in_seq) * tiles_b;
-        if (dec_split_is_aligned(p, s_prefix, segs_per_seq, total)) {
+        if (kKind != kMergePrefixFlat && dec_split_is_aligned(p, s_prefix, segs_per_seq, total)) {
             // the decode grid snapped its CTA boundaries to the segments: this segment's CTAs, of which
             // the first min(CTAs, tiles) have a piece
             c_first = dec_snap(t0, total, p.num_ctas);
@@ -96,15 +98,28 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 8 ? 4 : kWarps == 4 ? 8
         }
     }
     const int own_pieces = static_cast<int>(c_last - c_first + 1);
-    const int pieces = own_pieces + (kKind == kMergePrefix ? p.pre_parts : 0);
+    int pre_pieces = kKind == kMergePrefix ? p.pre_parts : 0;
+    const float *pre_o = nullptr, *pre_l = nullptr;   // kMergePrefixFlat: this row of the prefix's first piece
+    if (kKind == kMergePrefixFlat) {
+        const int rho = b * p.group + g, pseg = kvh * p.pre_blocks + rho / 16;
+        const long long t0 = own_total + static_cast<long long>(pseg) * p.pre_tiles;
+        const long long pc = cta_of_tile(total, p.num_ctas, t0);
+        pre_pieces = static_cast<int>(cta_of_tile(total, p.num_ctas, t0 + p.pre_tiles - 1) - pc + 1);
+        const long long slot = pc + p.batch * segs_per_seq + pseg;
+        pre_o = p.part_o + (slot * 16 + rho % 16) * kHeadDim + lane * 4;
+        pre_l = p.part_lse + slot * 16 + rho % 16;
+    }
+    const int pieces = own_pieces + pre_pieces;
     const float* lse_base = p.part_lse + (c_first + segment) * 16 + r;            // piece i at + i * 16
     const float* o_base = p.part_o + ((c_first + segment) * 16 + r) * kHeadDim + lane * 4;   // piece i at + i * 16 * 128
     auto piece_o = [&](int i) -> const float* {
         if (kKind == kMergePrefix && i >= own_pieces)
             return p.pre_o + ((i - own_pieces) * p.pre_rows + row) * kHeadDim + lane * 4;
+        if (kKind == kMergePrefixFlat && i >= own_pieces) return pre_o + static_cast<long long>(i - own_pieces) * 16 * kHeadDim;
         return o_base + static_cast<long long>(i) * 16 * kHeadDim;
     };
     auto piece_lse_at = [&](int i) -> const float* {
+        if (kKind == kMergePrefixFlat && i >= own_pieces) return pre_l + static_cast<long long>(i - own_pieces) * 16;
         if (kKind == kMergePrefix && i >= own_pieces) return p.pre_lse + (i - own_pieces) * p.pre_rows + row;
         return lse_base + static_cast<long long>(i) * 16;
     };

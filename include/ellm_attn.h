@@ -380,6 +380,9 @@ int ellm_attn_decode_noalloc(const void* q, const void* k_cache, const void* v_c
  *                           first.  Same cache bits either way.
  *   "tc_persistent"         prefill kernel: -1 (default) / 1 one CTA per SM walking the work-item list,
  *                           0 one CTA per item; a tuning knob.
+ *   "prefix_flat_mflops"    decode steps with a shared prefix: below this many MFLOP (4 x 128 x prefix_len x batch x
+ *                           query heads) the prefix goes through the split-KV kernel, from there on through the
+ *                           tensor-memory kernel; a tuning knob (0: always the latter).
  *   "decode_ctas"           grid of the decode kernel, 1 .. 2 x SMs (default 2 x SMs, for which the
  *                           workspace is sized); a tuning knob.
  * Unknown names return ELLM_ERR_INVALID_ARG.  The reference has no counterpart (it aborts). */
