@@ -111,7 +111,10 @@ __device__ __forceinline__ int dec_tiles_of(long long begin, long long len) {
 // kDecPrefix: a shared prefix, as segments (KV head, block of 16 of the step's query rows) behind the sequences' own
 // in the same tile list - the prefix is read once per 16 query rows, mostly from L2, by the one launch there
 // is anyway.  (Steps with more work take the tensor-memory kernel for the prefix, see launch_decode.)
-enum { kDecPlain = 0, kDecMods = 1, kDecPrefix = 2 };
+// kDecBehind: the launch right before is the tensor-memory kernel of the shared prefix, which lets this grid start once
+// everything before it has finished: nothing to wait for at the start, and the end waits for that kernel, so that
+// the merge behind this grid finds both.
+enum { kDecPlain = 0, kDecMods = 1, kDecPrefix = 2, kDecBehind = 3 };
 
 // kMods: the keys start at row_begin[b][position]; begs[b] receives that (where begs is given).
 template <bool kMods = false>
@@ -234,8 +237,10 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
     // Only then let the dependent grid (the merge) be set up: whatever it does before its own wait
     // - it rebuilds the tile table from the positions - then sees everything this grid sees.
     // With early streaming the wait comes later, after the first stages have been requested.
-    bool waited = p.early == 0;
-    if (waited) {
+    bool waited = p.early == 0 || kKind == kDecBehind;
+    if constexpr (kKind == kDecBehind) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    } else if (waited) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         ct.waited();
@@ -249,6 +254,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
                                ? dec_aligned_range(p, prefix, segs_per_seq, total, blockIdx.x, &t_begin, &t_end)
                                : assign_range(total, p.num_ctas, blockIdx.x, &t_begin, &t_end);
     if (!has_tiles) {
+        if constexpr (kKind == kDecBehind) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (!waited) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         return;
     }
@@ -479,6 +485,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
         __syncthreads();  // smem is reused by the next piece's ring
         t = piece_end;
     }
+    if constexpr (kKind == kDecBehind) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace ellm

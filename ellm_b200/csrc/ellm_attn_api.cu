@@ -379,6 +379,10 @@ int launch_decode(ellm_attn* h, const int32_t* positions, size_t position_index,
                 launch_dependent(ellm::decode_splitkv_kernel<2, ellm::kDecMods>, h->dec_ctas, ellm::kDecThreads, ellm::kDecModsSmemBytes, h->stream, p);
         } else if (merge_kind == ellm::kMergePrefixFlat)
             launch_dependent(ellm::decode_splitkv_kernel<2, ellm::kDecPrefix>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
+        else if (merge_kind == ellm::kMergePrefix && h->group <= 8)
+            launch_dependent(ellm::decode_splitkv_kernel<1, ellm::kDecBehind>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
+        else if (merge_kind == ellm::kMergePrefix)
+            launch_dependent(ellm::decode_splitkv_kernel<2, ellm::kDecBehind>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
         else if (h->group <= 8)   // blocks of 8 query heads per segment: one for groups of up to 8 heads, else two
             launch_dependent(ellm::decode_splitkv_kernel<1>, h->dec_ctas, ellm::kDecThreads, ellm::kDecSmemBytes, h->stream, p);
         else
@@ -608,6 +612,8 @@ int ellm_attn_create(const ellm_attn_desc* desc, ellm_attn** out) {
     if (cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, ellm::kDecPrefix>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1, ellm::kDecBehind>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, ellm::kDecBehind>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<1, ellm::kDecMods>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::decode_splitkv_kernel<2, ellm::kDecMods>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kDecModsSmemBytes) != cudaSuccess ||
         cudaFuncSetAttribute(ellm::prefill_warp_mma_kernel<__nv_bfloat16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kPfSmemBytes) != cudaSuccess ||

@@ -39,7 +39,8 @@
 // sequence), the keys the prefix alone, cut into `splits` runs of tiles so that every SM has work, and the
 // result is one fp32 partial (O, LSE) per run; the sequences' own keys go through the split-KV kernel and its
 // merge takes these partials in.  The prefix is read once per 256 query rows of a KV head instead of once per
-// sequence: with 64 sequences on 32768 keys the kernel is bound by the tensor core, with a handful by HBM.
+// sequence.  A K/V tile is used by one or two CTAs only, so the tiles come from HBM, where one TMA queue per SM
+// brings no more than about 20 GB/s: two further warps load them with 16-byte asynchronous copies instead.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -60,6 +61,8 @@ constexpr int kTcStages = 5;       // ring slots, each holds one K or one V tile
 constexpr int kTcTileBytes = kTcKeys * kRowBytes;          // 32 KB: two 16 KB halves of 128 rows x 128 B
 constexpr int kTcHalfBytes = kTcTileBytes / 2;
 constexpr int kTcThreads = (kTcTiles * 4 + 2) * 32;        // 320
+constexpr int kTcLoaders = 2;                              // kExtSplit: warps that copy K/V tiles, half a tile each
+constexpr int kTcSplitThreads = kTcThreads + kTcLoaders * 32;
 constexpr int kTcSmemQ = 0;
 constexpr int kTcSmemRing = kTcSmemQ + kTcTiles * kTcTileBytes;
 constexpr int kTcSmemBar = kTcSmemRing + kTcStages * kTcTileBytes;
@@ -840,7 +843,7 @@ __device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRo
 // separate instantiation, so that the plain kernel carries none of its state).
 // kExt: modified scores, intervals, shared prefix (map_kn / map_vn are then the prefix's maps).
 template <typename OutT, bool kFused, int kExt = 0>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__((kExt & kExtSplit) ? kTcSplitThreads : kTcThreads, 1)
 prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kn,
                        const __grid_constant__ CUtensorMap map_vn,
@@ -851,7 +854,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) { TC_TRACE_NS(0); TC_TRACE(1); }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr bool kSplit = (kExt & kExtSplit) != 0;
+    if constexpr (!kSplit) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == (kTcTiles * 4) * 32) {   // the producer thread fetches the three descriptors ahead of its first copy
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -890,14 +894,14 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             mbar_init(bar_pv_done(t), 1);
         }
         for (int s = 0; s < kTcStages; ++s) {
-            mbar_init(bar_kv_full(s), 1);
+            mbar_init(bar_kv_full(s), kSplit ? kTcLoaders : 1);
             mbar_init(bar_kv_empty(s), 1);
         }
         mbar_init(bar_tail, 1);
         mbar_init(bar_final, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_sched_full(i), 1);
-            mbar_init(bar_sched_empty(i), 1 + kTcTiles * 4);   // the MMA thread and every softmax warp
+            mbar_init(bar_sched_empty(i), 1 + kTcTiles * 4 + (kSplit ? kTcLoaders : 0));   // the MMA thread, every softmax and loader warp
         }
         *abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -915,6 +919,9 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // Launched as a programmatic dependent, the set-up above ran while the stream's previous kernel
     // was still at work; everything below reads or writes what that kernel may have touched.
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // the split-KV kernel behind this one reads nothing that this one writes: from here on it may run, and only
+    // its end waits for this grid's
+    if constexpr (kSplit) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) TC_TRACE(2);
     const int total_rows = p.interval * p.group;
     const int n_items = static_cast<int>(p.n_items);
@@ -1324,7 +1331,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                     pos0, it.kvh, it.b);
                     ++q_loads[t];
                 }
-                for (int item = 0; item < 2 * it.nsteps && ok; ++item, ++ring_n) {  // K_0, V_0, K_1, V_1, ...
+                for (int item = 0; !kSplit && item < 2 * it.nsteps && ok; ++item, ++ring_n) {  // K_0, V_0, K_1, V_1, ...
                     const int slot = static_cast<int>(ring_n % kTcStages);
                     const uint32_t round_par = static_cast<uint32_t>((ring_n / kTcStages) & 1);
                     if constexpr (kFused) {
@@ -1425,6 +1432,66 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             (void)tails;
         }
         __syncwarp();
+    } else if (kSplit && warp >= kTcTiles * 4 + 2) {
+        // =============================== K/V loaders (kExtSplit) ===============================
+        // Loader warp w copies rows [64 w, 64 w + 64) of every tile, 16 bytes a lane, a row's 256 contiguous bytes by
+        // 16 lanes, into the layout a TMA box of 128-byte swizzled rows has.  Up to four tiles are in flight; a tile
+        // is signalled (after the fence that makes it visible to the MMAs) when the copies of three later ones are out.
+        if constexpr (kSplit) {
+            constexpr int kAhead = 3;
+            const int half = warp - (kTcTiles * 4 + 2);
+            const int rlane = lane >> 4, chunk = lane & 15;
+            uint32_t off[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                off[i] = (chunk >> 3) * kTcHalfBytes + (half * 64 + 2 * i + rlane) * 128 + (((chunk & 7) ^ (2 * i + rlane)) << 4);
+            long long ring_n = 0, signalled = 0;
+            auto signal_upto = [&](long long n) {   // the copies of tiles < n have landed
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                for (; signalled < n; ++signalled)
+                    if (lane == 0 && signalled != p.debug_skip_item) mbar_arrive(bar_kv_full(static_cast<int>(signalled % kTcStages)));
+            };
+            bool ok = true;
+            Item it;
+            for (long long k = 0; ok; ++k) {
+                int idx = n_items;
+                if (lane == 0) idx = take_item(k, ok, kTcWaitSched);
+                idx = __shfl_sync(0xffffffffu, idx, 0);
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(bar_sched_empty(static_cast<int>(k & 1)));
+                if (idx >= n_items) break;
+                tc_item(p, idx, it);
+                const ScoreMods& m = p.ext.mods;
+                for (int item = 0; item < 2 * it.nsteps; ++item, ++ring_n) {
+                    const int slot = static_cast<int>(ring_n % kTcStages);
+                    if (lane == 0)
+                        ok = mbar_wait(bar_kv_empty(slot), static_cast<uint32_t>(((ring_n / kTcStages) & 1) ^ 1), abort_word, p.status, kTcWaitKvEmpty,
+                                       p.wait_timeout_ns);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                    if (!ok) break;
+                    const long long row0 = static_cast<long long>(it.p0 + (item >> 1)) * kTcKeys + half * 64 + rlane;
+                    const __nv_bfloat16* src = ((item & 1) ? m.pv : m.pk) + it.kvh * m.ps1 + row0 * m.ps2 + chunk * 8;
+                    const uint32_t dst = smem_base + kTcSmemRing + slot * kTcTileBytes;
+                    const long long left = m.plen - row0;   // row 2 i of this lane exists when 2 i < left
+                    if (left >= 64) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) cp_async_16(dst + off[i & 3] + (i >> 2) * 1024, src + i * 2 * m.ps2, 16);
+                    } else {
+#pragma unroll 4
+                        for (int i = 0; i < 32; ++i) cp_async_16(dst + off[i & 3] + (i >> 2) * 1024, 2 * i < left ? src + i * 2 * m.ps2 : m.pk, 2 * i < left ? 16 : 0);
+                    }
+                    cp_async_commit();
+                    cp_async_wait<kAhead>();
+                    if (ring_n >= kAhead) signal_upto(ring_n - kAhead + 1);
+                }
+                if (!ok) break;
+                cp_async_wait<0>();
+                signal_upto(ring_n);
+            }
+            cp_async_wait<0>();   // (a wait that ran out: nothing of this warp's is in flight when the block ends)
+        }
     } else {
         // =============================== MMA issuer ===============================
         // One thread issues every MMA, one GEMM after the other: two issuing threads were tried and
@@ -1827,7 +1894,7 @@ inline int launch_prefix_split(Tcgen05Plan& plan, const ellm_attn_desc& d, const
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(persistent ? std::min<long long>(p.n_items, plan.sm_count) : p.n_items));
-    cfg.blockDim = dim3(kTcThreads);
+    cfg.blockDim = dim3(kTcSplitThreads);
     cfg.dynamicSmemBytes = kTcSmemBytes;
     cfg.stream = stream;
     cfg.attrs = attr;
