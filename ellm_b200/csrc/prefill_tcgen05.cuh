@@ -1435,8 +1435,9 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (kSplit && warp >= kTcTiles * 4 + 2) {
         // =============================== K/V loaders (kExtSplit) ===============================
         // Loader warp w copies rows [64 w, 64 w + 64) of every tile, 16 bytes a lane, a row's 256 contiguous bytes by
-        // 16 lanes, into the layout a TMA box of 128-byte swizzled rows has.  Up to four tiles are in flight; a tile
-        // is signalled (after the fence that makes it visible to the MMAs) when the copies of three later ones are out.
+        // 16 lanes, into the layout a TMA box of 128-byte swizzled rows has.  Up to four tiles are in flight.  A tile is
+        // signalled, after the fence that makes it visible to the MMAs, when the copies of three later ones are
+        // out, or at once when there is no free slot to copy into: then the copies are ahead of the MMAs anyway.
         if constexpr (kSplit) {
             constexpr int kAhead = 3;
             const int half = warp - (kTcTiles * 4 + 2);
@@ -1466,9 +1467,13 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const ScoreMods& m = p.ext.mods;
                 for (int item = 0; item < 2 * it.nsteps; ++item, ++ring_n) {
                     const int slot = static_cast<int>(ring_n % kTcStages);
+                    const uint32_t par = static_cast<uint32_t>(((ring_n / kTcStages) & 1) ^ 1);
+                    if (signalled < ring_n && !__shfl_sync(0xffffffffu, lane == 0 ? mbar_try_wait(bar_kv_empty(slot), par) : 0u, 0)) {
+                        cp_async_wait<0>();
+                        signal_upto(ring_n);
+                    }
                     if (lane == 0)
-                        ok = mbar_wait(bar_kv_empty(slot), static_cast<uint32_t>(((ring_n / kTcStages) & 1) ^ 1), abort_word, p.status, kTcWaitKvEmpty,
-                                       p.wait_timeout_ns);
+                        ok = mbar_wait(bar_kv_empty(slot), par, abort_word, p.status, kTcWaitKvEmpty, p.wait_timeout_ns);
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                     if (!ok) break;
                     const long long row0 = static_cast<long long>(it.p0 + (item >> 1)) * kTcKeys + half * 64 + rlane;
@@ -1484,7 +1489,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                     cp_async_commit();
                     cp_async_wait<kAhead>();
-                    if (ring_n >= kAhead) signal_upto(ring_n - kAhead + 1);
+                    if (ring_n - kAhead + 1 > signalled) signal_upto(ring_n - kAhead + 1);
                 }
                 if (!ok) break;
                 cp_async_wait<0>();
