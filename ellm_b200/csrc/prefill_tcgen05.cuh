@@ -746,8 +746,30 @@ __device__ __forceinline__ float tc_row64(float (&s)[64], const TcRow& r, const 
     return 0.0f;
 }
 
-// The two-pass step of a kExt row tile: the true maximum, O_t rescaled to it where it moved far, then P.  Taken for a
-// row tile's first key tile and when a score leaps far above the maximum in use.  32 columns at a time in a rolled
+// The largest visible score of a key tile, for rows that have seen no key before it (they have l = 0 and nothing in
+// O_t, so the one-pass step can go on from it).  Rolled like the two-pass step.
+template <int kExt>
+__device__ __forceinline__ float tc_first_max(uint32_t tS, const TcRow& r, int lo, int rel) {
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld32(tS + c * 32, v);
+        tmem_wait_ld();
+        const int l0 = lo - c * 32, r0 = rel - c * 32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float x = (kExt & kExtBias) ? tc_score<kExt>(r, v[i], static_cast<float>(c * 32 + i)) : v[i];
+            mx = fmaxf(mx, i >= l0 && i <= r0 ? x : -INFINITY);
+        }
+    }
+    if constexpr ((kExt & kExtBias) == 0)
+        if (mx != -INFINITY) mx = tc_score<kExt>(r, mx, 0.0f);   // the score grows with the product
+    return mx;
+}
+
+// The two-pass step of a kExt row tile: the true maximum, O_t rescaled to it where it moved far, then P.  Taken when
+// a score leaps far above the maximum in use.  32 columns at a time in a rolled
 // loop: it is rare, and its code must not push the one-pass step's out of the instruction cache.
 template <int kExt>
 __device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRow& r, int lo, int rel, bool rescale_o, float& m_used, float& l) {
@@ -808,8 +830,12 @@ __device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRo
 template <int kExt>
 __device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRow& r, const float (&coef)[5], int lo, int rel, bool edge,
                                             bool first, bool fixed_max, bool valid, float& m_used, float& l) {
-    bool slow = first && !fixed_max;
-    if (!slow) {
+    bool slow = false;
+    if (!fixed_max && __any_sync(0xffffffffu, m_used == -INFINITY && valid)) {
+        const float m = tc_first_max<kExt>(tS, r, edge ? lo : 0, edge ? rel : 127);
+        if (m_used == -INFINITY) m_used = m;
+    }
+    {
         float sum0 = 0.0f;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
@@ -818,8 +844,8 @@ __device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRo
             tmem_ld32(tS + half * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
             tmem_wait_ld();
             uint32_t pk[32];
-            const float sum = tc_row64<kExt>(s, r, coef, static_cast<float>(half * 64), -m_used, edge, lo - half * 64, rel - half * 64, pk);
-            // a row that saw no key before this tile has m_used = -infinity: its first one shows up here too
+            const float sum = tc_row64<kExt>(s, r, coef, static_cast<float>(half * 64), m_used == -INFINITY ? 0.0f : -m_used, edge, lo - half * 64,
+                                             rel - half * 64, pk);   // (a row without any key yet: all masked)
             const bool leapt = !fixed_max && __any_sync(0xffffffffu, !(sum < kTcSumTrigger) && valid);
             if (!leapt) {
                 tmem_st32u(tS + half * 32, pk);
@@ -888,7 +914,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (threadIdx.x == 0) {
         for (int t = 0; t < kTcTiles; ++t) {
             mbar_init(bar_q(t), 1);
-            mbar_init(bar_q_empty(t), 1);
+            mbar_init(bar_q_empty(t), kSplit ? kTcTileRows / 32 : 1);   // (kExtSplit: the softmax warps, done with it as staging space)
             mbar_init(bar_s_full(t), 1);
             mbar_init(bar_p_full(t), kTcTileRows / 32);   // one arrival per softmax warp
             mbar_init(bar_pv_done(t), 1);
@@ -1208,6 +1234,37 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if constexpr (kExt != 0) {
                     if (!(l < INFINITY)) bad = true;
                 }
+                if constexpr (kSplit) {
+                    // A thread's row is 512 bytes: 16-byte stores of 32 threads would touch 32 lines each.  The warp turns
+                    // 64 columns of its 32 rows over in its quarter of the Q tile (which this item's products are done
+                    // with) and stores whole 256-byte runs.  Piece c of row r sits at c ^ (r & 15).
+                    unsigned char* stage = smem + kTcSmemQ + t * kTcTileBytes + (warp & 3) * (kTcTileBytes / 4);
+                    const unsigned live = __ballot_sync(0xffffffffu, valid);
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float o[32];
+                            tmem_ld32(tO + h * 64 + c * 32, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<float4*>(stage + lane * 256 + (((c * 8 + i) ^ (lane & 15)) << 4)) =
+                                    make_float4(o[i * 4 + 0] * inv, o[i * 4 + 1] * inv, o[i * 4 + 2] * inv, o[i * 4 + 3] * inv);
+                        }
+                        __syncwarp();
+#pragma unroll 4
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = 2 * i + (lane >> 4), c = lane & 15;
+                            const float4 v = *reinterpret_cast<const float4*>(stage + r * 256 + ((c ^ (r & 15)) << 4));
+                            const long long at = __shfl_sync(0xffffffffu, row_index, r);
+                            if ((live >> r) & 1u) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at * kHeadDim + h * 64 + c * 4) = v;
+                        }
+                        __syncwarp();
+                    }
+                    fence_async_smem();   // before the next item's Q may be copied in
+                    if (valid && p.lse) p.lse[row_index] = (m_used + log2f(l)) * kLn2;
+                } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float o[32];
@@ -1243,6 +1300,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     }
                 }
                 if (valid && p.lse) p.lse[row_index] = (m_used + log2f(l)) * kLn2;
+                }
                 if constexpr (kExt != 0 && sizeof(OutT) == 2) {
                     unsigned redo = __ballot_sync(0xffffffffu, bad && valid);
                     while (redo) {   // rare: one row at a time, the whole warp on it
@@ -1269,6 +1327,10 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(orow + i * 8) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 if (p.lse) p.lse[row_index] = -INFINITY;
+            }
+            if constexpr (kSplit) {
+                __syncwarp();
+                if (lane == 0 && my_steps > 0) mbar_arrive(bar_q_empty(t));
             }
             steps_done += my_steps;
             if ((warp & 3) == 0 && lane == 0) TC_TRACE(tr + 3);
@@ -1488,6 +1550,11 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         for (int i = 0; i < 32; ++i) cp_async_16(dst + off[i & 3] + (i >> 2) * 1024, 2 * i < left ? src + i * 2 * m.ps2 : m.pk, 2 * i < left ? 16 : 0);
                     }
                     cp_async_commit();
+                    if (item == 0) {   // the item's first K tile: everything waits for it
+                        cp_async_wait<0>();
+                        signal_upto(ring_n + 1);
+                        continue;
+                    }
                     cp_async_wait<kAhead>();
                     if (ring_n - kAhead + 1 > signalled) signal_upto(ring_n - kAhead + 1);
                 }
@@ -1557,7 +1624,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         for (int t = 0; t < kTcTiles; ++t)
                             if (it.steps[t] > 0) {
                                 issue_qk(t, slot_of(0));
-                                if (it.steps[t] == 1) umma_commit(bar_q_empty(t));   // this item reads Q_t no more
+                                if (!kSplit && it.steps[t] == 1) umma_commit(bar_q_empty(t));   // this item reads Q_t no more
                             }
                         umma_commit(bar_kv_empty(slot_of(0)));
                     }
@@ -1587,7 +1654,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                 tc_fence_after();
                             }
                             issue_qk(t, slot_k);
-                            if (j + 2 == it.steps[t]) umma_commit(bar_q_empty(t));
+                            if (!kSplit && j + 2 == it.steps[t]) umma_commit(bar_q_empty(t));
                         }
                     }
                     if (!ok) break;
