@@ -5,13 +5,14 @@
 #include "proj_tcgen05.cuh"
 #include "proj_skinny.cuh"
 #include "proj_w4.cuh"
+#include "proj_w4_tcgen05.cuh"
 
 struct ProjHandle {
     int which = 0;                 // 0 = MatMul3, 1 = MatMulAdd, 2 = MatMulAddW4
     ellm_matmul3_desc d3{};
     ellm_matmul_add_desc da{};
     ellm_matmul_add_w4_desc dw{};
-    __nv_bfloat16* w4_scratch = nullptr;    // MatMulAddW4, more than 16 rows: the weights as bf16, written by every such run
+    float* w4_part = nullptr;               // MatMulAddW4: parts of tiles cut between CTAs
     int device = 0;
     cudaStream_t stream = nullptr;
     bool async = false;
@@ -77,7 +78,7 @@ void proj_common_destroy(ProjHandle* h) {
     }
     cudaFree(h->status_dev);
     cudaFree(h->qkv_scratch);
-    cudaFree(h->w4_scratch);
+    cudaFree(h->w4_part);
     if (h->status_host) cudaFreeHost(h->status_host);
 }
 
@@ -523,6 +524,17 @@ W4Choice w4_choice_of(size_t group) {
 }
 // Warps across the columns and blocks per warp by the blocks a CTA has: one block leaves all 16 warps to K,
 // four and more put four warps across (a chunk of the rows then serves up to 16 blocks).
+// The tensor-memory form for `rows` per tile: exact up to 32, weights rounded to bf16 above.
+typedef void (*W4TcKernel)(const CUtensorMap, const uint8_t*, const ellm::W4TcParams);
+template <bool kSmall, int kMt>
+W4TcKernel w4_tc_kernel_of(size_t group) {
+    return group == 128 ? ellm::proj_w4_tcgen05_kernel<kSmall, kMt, 4> : group == 64 ? ellm::proj_w4_tcgen05_kernel<kSmall, kMt, 2>
+                                                                                     : ellm::proj_w4_tcgen05_kernel<kSmall, kMt, 1>;
+}
+W4TcKernel w4_tc_kernel(int mt, size_t group) {
+    return mt == 16 ? w4_tc_kernel_of<true, 16>(group) : mt == 32 ? w4_tc_kernel_of<true, 32>(group) : w4_tc_kernel_of<false, 0>(group);
+}
+
 template <int NB>
 W4Choice w4_choice(size_t n, size_t group, int sm_count) {
     const size_t blocks = ((n + 15) / 16 + sm_count - 1) / sm_count;
@@ -531,6 +543,14 @@ W4Choice w4_choice(size_t n, size_t group, int sm_count) {
     if (blocks <= 4) return w4_choice_of<1, 4, NB>(group);
     if (blocks <= 8) return w4_choice_of<2, 4, NB>(group);
     return w4_choice_of<4, 4, NB>(group);
+}
+
+// Up to 16 rows both forms give the same sums (to fp32).  The warp-level one is a single launch whose warps share a
+// column's K, the tensor-memory one unpacks with fewer instructions per weight but has to add up cut tiles in a
+// second launch.
+bool w4_use_tc(const ProjHandle* h, size_t rows) {
+    if (h->plan.pairing >= 0) return h->plan.pairing != 0;
+    return static_cast<long long>(h->dw.n_max) * static_cast<long long>(h->dw.k_max) * (rows > 8 ? 2 : 1) >= (1ll << 26);
 }
 
 }  // namespace
@@ -566,16 +586,15 @@ int ellm_matmul_add_w4_create(const ellm_matmul_add_w4_desc* d, ellm_matmul_add_
             if (cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, c.smem) != cudaSuccess)
                 st = fail(ELLM_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(cudaGetLastError()));
     }
-    if (st == ELLM_OK && d->m_max > static_cast<size_t>(ellm::kW4MaxRows)) {
-        if (cudaMalloc(&h->w4_scratch, d->n_max * d->k_max * 2) != cudaSuccess) {
+    if (st == ELLM_OK) {
+        for (const auto kernel : {w4_tc_kernel(16, d->group), w4_tc_kernel(32, d->group), w4_tc_kernel(256, d->group)})
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ellm::kWtSmemMax) != cudaSuccess)
+                st = fail(ELLM_ERR_CUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(cudaGetLastError()));
+        const size_t mt = std::min<size_t>(256, (d->m_max + 15) / 16 * 16), bytes = 2 * h->plan.sm_count * mt * ellm::kWtTileN * sizeof(float);
+        if (st == ELLM_OK && cudaMalloc(&h->w4_part, bytes) != cudaSuccess) {
             cudaGetLastError();
-            st = fail(ELLM_ERR_NO_MEMORY, "workspace allocation failed (%zu bytes)", d->n_max * d->k_max * 2);
-        } else if (!ellm::proj_encode_2d(h->plan, &h->map_w[0], h->w4_scratch, d->n_max, d->k_max, d->k_max, ellm::kPjBN) ||
-                   !ellm::proj_encode_2d(h->plan, &h->map_wp[0], h->w4_scratch, d->n_max, d->k_max, d->k_max, ellm::kPjBN / 2)) {
-            st = fail(ELLM_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled(weight) failed");
-        } else {
-            h->map_w[1] = h->map_w[2] = h->map_w[0];
-            h->map_wp[1] = h->map_wp[2] = h->map_wp[0];
+            h->w4_part = nullptr;
+            st = fail(ELLM_ERR_NO_MEMORY, "workspace allocation failed (%zu bytes)", bytes);
         }
     }
     if (st != ELLM_OK) {
@@ -612,7 +631,7 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
     const size_t lda = d.a_row_stride ? d.a_row_stride : d.k_max;
     const long long ldc = static_cast<long long>(d.output_row_stride ? d.output_row_stride : d.n_max);
     const long long ldr = static_cast<long long>(d.residual_row_stride ? d.residual_row_stride : d.n_max);
-    if (rows <= static_cast<size_t>(ellm::kW4MaxRows)) {
+    if (rows <= static_cast<size_t>(ellm::kW4MaxRows) && !w4_use_tc(h, rows)) {
         ellm::W4Params p{};
         p.a = static_cast<const __nv_bfloat16*>(d.a);
         p.lda = static_cast<long long>(lda);
@@ -634,23 +653,53 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
         ++h->skinny_launches;
         return proj_finish(h);
     }
-    const long long words = static_cast<long long>(d.n_max) * static_cast<long long>(d.k_max / 8);
-    const unsigned blocks = static_cast<unsigned>(std::min<long long>((words + 255) / 256, 8ll * h->plan.sm_count));
-    ELLM_CUDA(launch_dependent(ellm::w4_unpack_kernel, blocks, 256, 0, h->stream, static_cast<const uint32_t*>(d.w4),
-                               static_cast<const __nv_bfloat16*>(d.scales), static_cast<const uint8_t*>(d.zeros),
-                               reinterpret_cast<uint4*>(h->w4_scratch), words, static_cast<int>(d.k_max / 8), static_cast<int>(d.group / 8)));
-    ++h->skinny_launches;
-    ellm::ProjParams p{};
-    p.mode = ellm::kPjPlain;
-    p.tiles_n = static_cast<int>((d.n_max + ellm::kPjBN - 1) / ellm::kPjBN);
+    const size_t tiles_m = rows <= 32 ? 1 : (rows + 255) / 256;
+    const int mt = rows <= 16 ? 16 : rows <= 32 ? 32 : static_cast<int>(((rows + tiles_m - 1) / tiles_m + 15) / 16 * 16);
+    if (h->map_a_rows != rows) {
+        if (!ellm::proj_encode_2d(h->plan, &h->map_a, d.a, rows, d.k_max, lda, static_cast<unsigned>(mt)))
+            return fail(ELLM_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled(A) failed");
+        h->map_a_rows = rows;
+    }
+    ellm::W4TcParams p{};
+    p.scales = static_cast<const __nv_bfloat16*>(d.scales);
+    p.zeros = static_cast<const uint8_t*>(d.zeros);
+    p.residual = static_cast<const __nv_bfloat16*>(d.residual);
+    p.c = static_cast<__nv_bfloat16*>(d.output);
+    p.ldr = ldr;
+    p.ldc = ldc;
+    p.part = h->w4_part;
+    p.status = h->status_dev;
+    p.wait_timeout_ns = h->plan.wait_timeout_ns;
+    p.debug_skip_load = h->plan.debug_skip_load;
+    p.m_rows = static_cast<int>(rows);
     p.batch = static_cast<int>(batch_size);
     p.max_batch = static_cast<int>(d.max_batch);
-    p.c = static_cast<__nv_bfloat16*>(d.output);
-    p.residual = static_cast<const __nv_bfloat16*>(d.residual);
-    p.ldc = ldc;
-    p.ldr = ldr;
     p.n_cols = static_cast<int>(d.n_max);
-    return proj_launch(h, d.a, lda, d.k_max, rows, p);
+    p.blocks = static_cast<int>(d.k_max / 128);
+    p.tiles_m = static_cast<int>((rows + mt - 1) / mt);
+    p.mt = mt;
+    p.stages = ellm::w4_tc_stages(mt);
+    const long long tiles = static_cast<long long>((d.n_max + ellm::kWtTileN - 1) / ellm::kWtTileN) * p.tiles_m;
+    p.units = tiles * p.blocks;
+    if (p.units > 0x7fffffffll) return fail(ELLM_ERR_UNSUPPORTED, "too many tiles for one launch");
+    const unsigned ctas = static_cast<unsigned>(std::min<long long>(p.units, h->plan.sm_count));
+    ELLM_CUDA(launch_dependent(w4_tc_kernel(mt, d.group), ctas, ellm::kWtThreads, static_cast<size_t>(ellm::w4_tc_smem(mt)), h->stream, h->map_a,
+                               static_cast<const uint8_t*>(d.w4), p));
+    ++h->launches;
+    if (p.units % ctas != 0 || (p.units / ctas) % p.blocks != 0) {   // some tile is cut
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attrs[1];
+        attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((mt + 7) / 8));
+        cfg.blockDim = dim3(128);
+        cfg.stream = h->stream;
+        cfg.attrs = attrs;
+        cfg.numAttrs = 1;
+        ELLM_CUDA(cudaLaunchKernelEx(&cfg, ellm::w4_reduce_kernel, p, static_cast<int>(ctas)));
+        ++h->launches;
+    }
+    return proj_finish(h);
 }
 
 static ProjHandle* proj_cast(void* handle, int which) {

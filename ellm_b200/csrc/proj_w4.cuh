@@ -21,9 +21,7 @@
 //     (q - z) * x.  The detour costs at most (16 + 15) / 1 of a rounding of fp32: 2e-6 of sum |x| |q - z|.
 // The sums of the WK warps of a column are added in warp order: the result does not depend on timing.
 //
-// More rows: w4_unpack_kernel writes the weights once as bf16 (this rounds (q - z) * scale to 8 bits, half
-// a bf16 step per weight; unlike above the tensor-memory accumulator runs over all groups, so the scale
-// has to be in the operand) and proj_tcgen05_kernel multiplies.
+// Large weights and more rows: proj_w4_tcgen05.cuh.
 #pragma once
 #include "common.cuh"
 
@@ -356,26 +354,6 @@ __global__ void __launch_bounds__(W4Shape<CB, WN, NB>::kThreads, 1) proj_w4_kern
             p.c[m * p.ldc + n] = __float2bfloat16_rn(sum);
         }
         if (pass + 1 < passes) __syncthreads();
-    }
-}
-
-// Packed weights -> bf16 [n][k]; a thread unpacks 8 inputs.  HBM-bound: 0.5 byte read, 2 written per weight.
-__global__ void __launch_bounds__(256) w4_unpack_kernel(const uint32_t* w, const __nv_bfloat16* scales, const uint8_t* zeros, uint4* out,
-                                                        long long words, int words_row, int words_group) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int groups_row = words_row / words_group;
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < words; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const long long n = i / words_row;
-        const long long at = n * groups_row + static_cast<int>(i - n * words_row) / words_group;
-        const float s = __bfloat162float(scales[at]);
-        const float zs = static_cast<float>(zeros ? zeros[at] : 8);
-        const uint32_t word = w[i];
-        uint32_t r[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            r[j] = pack_bf16((static_cast<float>((word >> (8 * j)) & 15u) - zs) * s, (static_cast<float>((word >> (8 * j + 4)) & 15u) - zs) * s);
-        out[i] = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
 

@@ -166,7 +166,9 @@ int ellm_matmul_check(void* handle, int which);
 int ellm_matmul_set_wait_timeout(void* handle, int which, unsigned long long ns);
 /* Tuning knob of the tensor-memory kernel: two CTAs of a cluster share a 256 x 256 tile
  * (tcgen05 cta_group::2; each CTA loads its 128 rows of A and half of the weight tile).
- * mode -1 (default): when every pair gets at least two tiles; 0: never; 1: whenever rows > 128. */
+ * mode -1 (default): when every pair gets at least two tiles; 0: never; 1: whenever rows > 128.
+ * Of a `which` 2 handle: which kernel takes runs of at most 16 rows, 0 the warp-level one, 1 the
+ * tensor-memory one, -1 (default) by the size of the weights. */
 int ellm_matmul_set_pairing(void* handle, int which, int mode);
 /* Test hook for the failure path: the tensor-memory kernel's loader leaves operand block `item`
  * (counted over the first CTA's k-blocks) unloaded, so the wait on it runs out after the bound above

@@ -18,18 +18,19 @@ def make(seed, rows, n, k, group, zeros, residual, max_batch=None, dev="cuda:0",
     return [t.to(dev) if t is not None else None for t in (q, scales, z, a, r)]
 
 
-def run(seed, rows, n, k, group, zeros=True, residual=True, pad=0, live=None, chunk=False):
+def run(seed, rows, n, k, group, zeros=True, residual=True, pad=0, live=None, chunk=False, kernel=-1):
     from ellm_b200 import MatMulAddW4, pack_int4
     q, scales, z, a, r = make(seed, rows, n, k, group, zeros, residual, pad=pad)
     out = torch.full((rows, n + pad), 7.0, dtype=torch.bfloat16, device=a.device)
     op = MatMulAddW4.new(a, pack_int4(q), scales, r, out, rows, n, k, group, zeros=z, a_row_stride=k + pad,
                          residual_row_stride=n + pad, output_row_stride=n + pad, max_batch=1 if chunk else rows)
+    op.set_pairing(kernel)
     live = rows if live is None else live
     op.run(0, *((live, 1) if chunk else (1, live)))
     torch.cuda.synchronize()
     op.close()
     w = w4_weights(q, scales, z, group)
-    assert_w4(out[:live, :n], a[:live, :k], w, r[:live, :n] if residual else None, rounded_weights=live > 16 or (rows > 16 and not chunk))
+    assert_w4(out[:live, :n], a[:live, :k], w, r[:live, :n] if residual else None, rounded_weights=live > 32 or (rows > 32 and not chunk))
     assert bool((out[live:] == 7.0).all()) and bool((out[:, n:] == 7.0).all())
 
 
@@ -37,36 +38,47 @@ def run(seed, rows, n, k, group, zeros=True, residual=True, pad=0, live=None, ch
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16])
 @pytest.mark.parametrize("zeros,residual", [(False, False), (True, True)])
-def test_few_rows(group, rows, zeros, residual):
-    run(1, rows, 264, 1024, group, zeros, residual)
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_few_rows(group, rows, zeros, residual, kernel):
+    run(1, rows, 264, 1024, group, zeros, residual, kernel=kernel)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,k", [(8, 128), (16, 256), (40, 384), (2368, 640), (4744, 512), (5120, 2048), (9480, 1152), (30000, 256)], ids=str)
 @pytest.mark.parametrize("rows", [1, 13])
-def test_few_rows_sizes(n, k, rows):
-    run(2, rows, n, k, 64 if k % 256 else 32)
-    run(3, rows, n, k, 128, zeros=False, residual=False)
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_few_rows_sizes(n, k, rows, kernel):
+    run(2, rows, n, k, 64 if k % 256 else 32, kernel=kernel)
+    run(3, rows, n, k, 128, zeros=False, residual=False, kernel=kernel)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [17, 100, 300])
-@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("rows", [17, 32, 33, 100, 256, 257, 300, 700])
+@pytest.mark.parametrize("group", [32, 64, 128])
 def test_many_rows(rows, group):
     run(4, rows, 520, 768, group, chunk=True)
     run(5, rows, 256, 384, group, zeros=False, residual=False)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [5, 16, 40])
-def test_strides_and_idle_rows(rows):
-    run(6, rows, 136, 256, 64, pad=24)
-    run(7, rows, 136, 256, 64, live=rows - 3)
-    run(8, rows, 136, 256, 64, live=rows - 3, chunk=True)
+@pytest.mark.parametrize("rows", [16, 40, 513])
+@pytest.mark.parametrize("n,k", [(8, 128), (128, 128), (19000, 128), (136, 8192), (9480, 640)], ids=str)
+def test_tiles_cut_between_ctas(rows, n, k):
+    run(6, rows, n, k, 128, kernel=1, chunk=True)
 
 
 @pytest.mark.gpu
-def test_extreme_weights_are_exact():
+@pytest.mark.parametrize("rows", [5, 16, 40])
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_strides_and_idle_rows(rows, kernel):
+    run(6, rows, 136, 256, 64, pad=24, kernel=kernel)
+    run(7, rows, 136, 256, 64, live=rows - 3, kernel=kernel)
+    run(8, rows, 136, 256, 64, live=rows - 3, chunk=True, kernel=kernel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_extreme_weights_are_exact(kernel):
     """All 16 numbers, zero points 0 and 15, one-hot rows: the products come out as (q - z) * scale rounded once."""
     from ellm_b200 import MatMulAddW4, pack_int4
     dev = "cuda:0"
@@ -79,6 +91,7 @@ def test_extreme_weights_are_exact():
         a[torch.arange(16), i0 + torch.arange(16)] = 1.0
         out = torch.zeros(16, n, dtype=torch.bfloat16, device=dev)
         op = MatMulAddW4.new(a, pack_int4(q), scales, None, out, 16, n, k, 32, zeros=z)
+        op.set_pairing(kernel)
         op.run(0, 1, 16)
         torch.cuda.synchronize()
         op.close()
@@ -87,7 +100,8 @@ def test_extreme_weights_are_exact():
 
 
 @pytest.mark.gpu
-def test_results_do_not_depend_on_timing_and_the_output_may_be_the_residual():
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_results_do_not_depend_on_timing_and_the_output_may_be_the_residual(kernel):
     from ellm_b200 import MatMulAddW4, pack_int4
     q, scales, z, a, r = make(9, 11, 1032, 4096, 64, True, True)
     w4 = pack_int4(q)
@@ -95,6 +109,7 @@ def test_results_do_not_depend_on_timing_and_the_output_may_be_the_residual():
     for _ in range(5):
         y = r.clone()
         op = MatMulAddW4.new(a, w4, scales, y, y, 11, 1032, 4096, 64, zeros=z)
+        op.set_pairing(kernel)
         op.run(0, 1, 11)
         torch.cuda.synchronize()
         op.close()
@@ -123,7 +138,7 @@ def test_captured_and_replayed_with_new_inputs_and_weights(rows):
         w4.copy_(pack_int4(q))
         graph.replay()
         stream.synchronize()
-    assert_w4(out, a, w4_weights(q, scales, z, 128), r, rows > 16)
+    assert_w4(out, a, w4_weights(q, scales, z, 128), r, rows > 32)
     op.check()
     del graph
     op.close()
@@ -150,6 +165,27 @@ def test_refusals():
     with pytest.raises(ValueError):                        # not on the GPU
         new(w4_ptr=w)
     assert pack_int4(torch.tensor([[1, 2, 15, 0]], dtype=torch.uint8)).tolist() == [[0x21, 0x0F]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [16, 80])
+def test_a_load_that_never_comes_is_reported_and_the_handle_goes_on(rows):
+    from ellm_b200 import EllmError, MatMulAddW4, pack_int4
+    from ellm_b200 import _lib as L
+    q, scales, z, a, r = make(12, rows, 256, 1024, 128, True, True)
+    out = torch.zeros(rows, 256, dtype=torch.bfloat16, device="cuda:0")
+    op = MatMulAddW4.new(a, pack_int4(q), scales, r, out, rows, 256, 1024, 128, zeros=z)
+    op.set_pairing(1)
+    op.set_wait_timeout(20_000_000)
+    op.debug_skip_load(0)
+    with pytest.raises(EllmError) as e:
+        op.run(0, 1, rows)
+    assert e.value.status == L.ERR_DEVICE_TIMEOUT
+    op.debug_skip_load(-1)
+    op.run(0, 1, rows)
+    torch.cuda.synchronize()
+    assert_w4(out, a, w4_weights(q, scales, z, 128), r, rows > 32)
+    op.close()
 
 
 @pytest.mark.gpu
