@@ -547,10 +547,11 @@ W4Choice w4_choice(size_t n, size_t group, int sm_count) {
 
 // Up to 16 rows both forms give the same sums (to fp32).  The warp-level one is a single launch whose warps share a
 // column's K, the tensor-memory one unpacks with fewer instructions per weight but has to add up cut tiles in a
-// second launch.
+// second launch.  Measured (us, warp-level / tensor-memory): 8192 x 8192, 8 rows 20.1 / 22.9, 13 rows 27.3 / 23.0;
+// 28672 x 8192, 8 rows 57.8 / 55.8, 13 rows 69.5 / 56.0; 5120 x 2048, 13 rows 8.5 / 11.9.
 bool w4_use_tc(const ProjHandle* h, size_t rows) {
     if (h->plan.pairing >= 0) return h->plan.pairing != 0;
-    return static_cast<long long>(h->dw.n_max) * static_cast<long long>(h->dw.k_max) * (rows > 8 ? 2 : 1) >= (1ll << 26);
+    return static_cast<long long>(h->dw.n_max) * static_cast<long long>(h->dw.k_max) * (rows > 8 ? 4 : 1) >= (1ll << 27);
 }
 
 }  // namespace

@@ -5,14 +5,15 @@
 //
 // What bounds it: up to 32 rows the packed weights from HBM (0.5 byte each); with a prompt chunk the products.
 // In between stands the unpacking, about 14 instructions per 8 weights, done once per weight and row tile.
-//   warps 0-7   unpack: a warp has 16 weight rows, a thread one of them and 64 of the block's 128 inputs.  The warp
-//               streams its packed words through a private ring of 16-byte asynchronous copies (by TMA a block is
-//               128 requests of 64 bytes, of which too few are in flight: 2000 clocks a block, whatever the rest
-//               did) and writes bf16 into the 128-byte-swizzled tile the MMA reads
+//   warps 0-7   unpack: two groups of four, one block each in turn; a thread has one weight row.  A warp streams its
+//               32 rows' packed words through a private ring of 16-byte asynchronous copies (a TMA box of 128 x 64 bytes
+//               is 128 requests, of which too few are in flight) and stores the bf16 pairs into tensor memory, where the
+//               MMA takes its A operand from: no shared-memory round trip and no proxy fence (300 clocks a block)
 //   warp  8     TMA producer of the rows (m x 256 bytes per 128-input block)
 //   warp  9     MMA issuer, owner of tensor memory
 //   warps 10-13 drain / epilogue: thread = one weight row
-// kSmall (up to 32 rows): the tile holds q - z, exact in bf16, every group of a block has its own accumulator columns,
+// Tensor memory: columns [0, 256) four unpacked blocks (128 rows x 128 inputs each), [256, 512) accumulators.
+// kSmall (up to 32 rows): a block holds q - z, exact in bf16, every group of a block has its own accumulator columns,
 // and the drain warps add scale * accumulator to fp32 sums in registers: no rounding but the last.  Otherwise the tile
 // holds (q - z) * scale rounded to bf16 (half a step per weight) and tensor memory accumulates over all of K.
 // Work split: the (tile, 128-input block) units form one list, cut evenly over one CTA per SM.  A tile that falls to
@@ -25,13 +26,10 @@ namespace ellm {
 
 constexpr int kWtThreads = 14 * 32;
 constexpr int kWtTileN = 128;
-constexpr int kWtPacked = kWtTileN * 64;               // a block's packed weights: 8 KB
-constexpr int kWtUnpacked = kWtTileN * 256;            // as bf16: two 16 KB halves of 64 inputs
-constexpr int kWtUnpackedBufs = 2;
+constexpr int kWtWarpPacked = 32 * 64;                 // a warp's packed weights of a block: 2 KB
 constexpr int kWtMaxStages = 8;
 constexpr int kWtSmemMax = 232448;
-constexpr int kWtSmemFixed = kWtUnpackedBufs * kWtUnpacked + 512 + 1024;   // + barriers, + slack to align the base to 1024
-constexpr int kWtRingSmall = 12, kWtRing = 3;          // blocks of packed weights in flight (kSmall / many rows)
+constexpr int kWtRingSmall = 7, kWtRing = 2;           // slots of a warp's ring (kSmall / many rows)
 
 enum { kWtWaitIn = 21, kWtWaitInEmpty = 22, kWtWaitUnpacked = 23, kWtWaitUnpackedEmpty = 24, kWtWaitAcc = 25, kWtWaitAccEmpty = 26 };
 
@@ -52,7 +50,8 @@ struct W4TcParams {
     int stages;                    // ring of row blocks
 };
 
-inline int w4_tc_fixed(int mt) { return kWtSmemFixed + (mt <= 32 ? kWtRingSmall : kWtRing) * kWtPacked; }
+// packed rings, barriers, slack to align the base to 1024
+inline int w4_tc_fixed(int mt) { return (mt <= 32 ? kWtRingSmall : kWtRing) * 8 * kWtWarpPacked + 512 + 1024; }
 inline int w4_tc_stages(int mt) {
     const int s = (kWtSmemMax - w4_tc_fixed(mt)) / (mt * 256), most = mt <= 32 ? 4 : kWtMaxStages;
     return s > most ? most : s;
@@ -76,6 +75,13 @@ __device__ __forceinline__ bool w4_segment(const W4TcParams& p, long long u, lon
     s.whole = s.blocks == p.blocks;
     s.slot = 2 * static_cast<int>(blockIdx.x) + (u == u0 ? 0 : 1);
     return true;
+}
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 // 8 weights of a word as four bf16 pairs in input order, (q - z) exactly, times s2 when kScale.  16 + q is the byte
@@ -109,17 +115,16 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
     const int mt = kSmall ? kMt : p.mt;
     const int stage_bytes = mt * 256;
     constexpr int kRing = kSmall ? kWtRingSmall : kWtRing;
-    // [unpacked tiles][row stages][packed weights: kRing x 1 KB per unpack warp][barriers]
-    const uint32_t s_un = base, s_in = base + kWtUnpackedBufs * kWtUnpacked, s_packed = s_in + p.stages * stage_bytes,
-                   bar0 = s_packed + kRing * kWtPacked;
+    // [row stages][packed weights: kRing x 2 KB per unpack warp][barriers]
+    const uint32_t s_in = base, s_packed = s_in + p.stages * stage_bytes, bar0 = s_packed + kRing * 8 * kWtWarpPacked;
     auto bar_in = [&](int s) { return bar0 + 8u * s; };
     auto bar_in_empty = [&](int s) { return bar0 + 8u * (kWtMaxStages + s); };
-    auto bar_un = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + b); };
-    auto bar_un_empty = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 2 + b); };
-    auto bar_acc = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 4 + b); };
-    auto bar_acc_empty = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 6 + b); };
-    const uint32_t bar_final = bar0 + 8u * (2 * kWtMaxStages + 8);
-    unsigned char* tail = smem + (bar0 - base) + 8 * (2 * kWtMaxStages + 9);
+    auto bar_un = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + b); };                // unpacked block b of four
+    auto bar_un_empty = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 4 + b); };
+    auto bar_acc = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 8 + b); };
+    auto bar_acc_empty = [&](int b) { return bar0 + 8u * (2 * kWtMaxStages + 10 + b); };
+    const uint32_t bar_final = bar0 + 8u * (2 * kWtMaxStages + 12);
+    unsigned char* tail = smem + (bar0 - base) + 8 * (2 * kWtMaxStages + 14);
     volatile int* abort_word = reinterpret_cast<volatile int*>(tail);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8);
 
@@ -128,9 +133,11 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
             mbar_init(bar_in(s), 1);
             mbar_init(bar_in_empty(s), 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(bar_un(b), 8);
+        for (int b = 0; b < 4; ++b) {
+            mbar_init(bar_un(b), 4);
             mbar_init(bar_un_empty(b), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
             mbar_init(bar_acc(b), 1);
             mbar_init(bar_acc_empty(b), 4);
         }
@@ -156,72 +163,80 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
 
     if (warp < 8) {
         // =============================== unpack ===============================
-        const int rw = lane & 15, r = warp * 16 + rw, half = lane >> 4;   // weight row of the tile, half of the block's inputs
-        unsigned char* ring = smem + (s_packed - base) + warp * kRing * 1024;
+        // group = warp / 4 takes every other unit of the CTA's run; this thread's row = its tensor-memory lane
+        const int group = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        unsigned char* ring = smem + (s_packed - base) + warp * kRing * kWtWarpPacked;
         // 64-byte row segments; piece c of row i sits at c ^ ((i >> 1) & 3).  A lane copies piece lane & 3 of rows
-        // lane / 4 and lane / 4 + 8 of the warp's 16.
+        // lane / 4 + 8 i of the warp's 32.
         const int pr = lane >> 2, pc = lane & 3;
         const uint32_t pdst = smem_u32(ring) + pr * 64 + ((pc ^ ((pr >> 1) & 3)) << 4);
-        const long long row_bytes = static_cast<long long>(p.blocks) * 64;
-        long long iu = u0;           // the next unit to be requested: its row tile, block, weight row of this lane
+        const long long row_bytes = static_cast<long long>(p.blocks) * 64, step8 = 8 * row_bytes;
+        // the next unit to be requested: its block, row tile, weight row of this lane
+        long long iu = u0;
         int islot = 0, iblock = 0, im = 0, in = 0;
         const uint8_t* isrc = w4;
         if (u0 < u1) {
             const long long tile = u0 / p.blocks;
             iblock = static_cast<int>(u0 - tile * p.blocks);
             im = static_cast<int>(tile % p.tiles_m);
-            in = static_cast<int>(tile / p.tiles_m) * kWtTileN + warp * 16 + pr;
+            in = static_cast<int>(tile / p.tiles_m) * kWtTileN + (warp & 3) * 32 + pr;
             isrc = w4 + in * row_bytes + iblock * 64 + pc * 16;
         }
+        auto advance = [&]() {
+            ++iu;
+            isrc += 64;
+            if (++iblock == p.blocks) {   // the next tile: the same weights for the next row tile, or the next 128
+                iblock = 0;
+                isrc -= row_bytes;
+                if (++im == p.tiles_m) {
+                    im = 0;
+                    in += kWtTileN;
+                    isrc += kWtTileN * row_bytes;
+                }
+            }
+        };
         auto issue = [&]() {
             if (iu < u1) {
-                const bool a = in < p.n_cols, b = in + 8 < p.n_cols;   // rows that do not exist: zeros
-                cp_async_16(pdst + islot * 1024, a ? isrc : w4, a ? 16 : 0);
-                cp_async_16(pdst + islot * 1024 + 512, b ? isrc + 8 * row_bytes : w4, b ? 16 : 0);
-                ++iu;
-                islot = islot + 1 == kRing ? 0 : islot + 1;
-                isrc += 64;
-                if (++iblock == p.blocks) {   // the next tile: the same weights for the next row tile, or the next 128
-                    iblock = 0;
-                    isrc -= row_bytes;
-                    if (++im == p.tiles_m) {
-                        im = 0;
-                        in += kWtTileN;
-                        isrc += kWtTileN * row_bytes;
-                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {   // rows that do not exist: zeros
+                    const bool a = in + i * 8 < p.n_cols;
+                    cp_async_16(pdst + islot * kWtWarpPacked + i * 512, a ? isrc + i * step8 : w4, a ? 16 : 0);
                 }
+                islot = islot + 1 == kRing ? 0 : islot + 1;
+                advance();
+                if (iu < u1) advance();
             }
             cp_async_commit();
         };
+        if (group == 1 && iu < u1) advance();
 #pragma unroll 1
         for (int i = 0; i < kRing - 1; ++i) issue();
+        // zero points and scales of this thread's row, requested one of its blocks ahead
+        uint32_t z_next[kGroups];
+        __nv_bfloat16 s_next[kGroups];
+        auto fetch = [&](int tile_n, int block) {
+            const int n = min(tile_n * kWtTileN + r, p.n_cols - 1);
+            const long long at = (static_cast<long long>(n) * p.blocks + block) * kGroups;
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                z_next[g] = p.zeros ? p.zeros[at + g] : 8u;
+                if (!kSmall) s_next[g] = p.scales[at + g];
+            }
+        };
         int slot = 0;
-        unsigned n_done = 0;
+        unsigned n_done = 0;      // units of the CTA's run
         bool ok = true;
         for (long long u = u0; ok && w4_segment(p, u, u0, u1, sg); u += sg.blocks) {
-            const int n = min(sg.tile_n * kWtTileN + r, p.n_cols - 1);
-            // the groups of this thread's 64 inputs: one (of 64 or 128) or two (of 32)
-            constexpr int kMine = kGW == 1 ? 2 : 1;
-            const long long at0 = static_cast<long long>(n) * p.blocks * kGroups + (kGW == 4 ? 0 : half * kMine);
-            // (zero points and scales are requested a block ahead: two dependent trips to L2 otherwise)
-            uint32_t z_next[kMine];
-            __nv_bfloat16 s_next[kMine];
-            auto fetch = [&](int block) {
-                const long long at = at0 + static_cast<long long>(block) * kGroups;
-#pragma unroll
-                for (int g = 0; g < kMine; ++g) {
-                    z_next[g] = p.zeros ? p.zeros[at + g] : 8u;
-                    if (!kSmall) s_next[g] = p.scales[at + g];
-                }
-            };
-            fetch(sg.block0);
+            bool have = false;    // the requested zero points are of this segment
             for (int j = 0; j < sg.blocks && ok; ++j, ++n_done) {
-                uint32_t z16[kMine], s2[kMine];
+                if ((n_done & 1u) != static_cast<unsigned>(group)) continue;
+                if (!have) fetch(sg.tile_n, sg.block0 + j);
+                have = true;
+                uint32_t z16[kGroups], s2[kGroups];
 #pragma unroll
-                for (int g = 0; g < kMine; ++g) {
-                    const uint32_t z = z_next[g];
-                    // 16 + z in bf16 (z up to 127: exact): below 112 it is 16 + z < 128
-                    const __nv_bfloat162 zz = __float2bfloat162_rn(16.0f + static_cast<float>(z));
+                for (int g = 0; g < kGroups; ++g) {
+                    const __nv_bfloat162 zz = __float2bfloat162_rn(16.0f + static_cast<float>(z_next[g]));   // exact (z up to 127)
                     z16[g] = *reinterpret_cast<const uint32_t*>(&zz);
                     s2[g] = 0u;
                     if (!kSmall) {
@@ -229,28 +244,36 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                         s2[g] = *reinterpret_cast<const uint32_t*>(&ss);
                     }
                 }
-                if (j + 1 < sg.blocks) fetch(sg.block0 + j + 1);
+                if (j + 2 < sg.blocks) fetch(sg.tile_n, sg.block0 + j + 2);
                 issue();
                 cp_async_wait<kRing - 1>();
                 __syncwarp();
-                const unsigned char* wp = ring + slot * 1024 + rw * 64;
-                uint4 w[2];
+                const unsigned char* wp = ring + slot * kWtWarpPacked + lane * 64;
+                uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) w[i] = *reinterpret_cast<const uint4*>(wp + (((half * 2 + i) ^ ((rw >> 1) & 3)) << 4));
+                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(wp + ((i ^ ((lane >> 1) & 3)) << 4));
                 slot = slot + 1 == kRing ? 0 : slot + 1;
-                const int b = static_cast<int>(n_done & 1);
+                const int b = static_cast<int>(n_done & 3);
                 if (lane == 0)
-                    ok = mbar_wait(bar_un_empty(b), static_cast<uint32_t>(((n_done >> 1) & 1) ^ 1), abort_word, p.status, kWtWaitUnpackedEmpty, p.wait_timeout_ns);
+                    ok = mbar_wait(bar_un_empty(b), ((n_done >> 2) & 1u) ^ 1u, abort_word, p.status, kWtWaitUnpackedEmpty, p.wait_timeout_ns);
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;   // (also: every lane has read its packed words)
                 if (!ok) break;
-                unsigned char* dst = smem + b * kWtUnpacked + half * (kWtUnpacked / 2) + r * 128;
+                tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {   // 8 words of 8 inputs
-                    const uint32_t word = (i & 3) == 0 ? w[i >> 2].x : (i & 3) == 1 ? w[i >> 2].y : (i & 3) == 2 ? w[i >> 2].z : w[i >> 2].w;
-                    const int g = kGW == 1 ? i >> 2 : 0;
-                    *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = w4_unpack8<!kSmall>(word, z16[g], s2[g]);
+                for (int h = 0; h < 2; ++h) {   // 64 inputs: 32 columns
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint4& v = w[h * 2 + (i >> 2)];
+                        const uint32_t word = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+                        const int g = (h * 2 + (i >> 2)) / kGW;
+                        const uint4 o = w4_unpack8<!kSmall>(word, z16[g], s2[g]);
+                        pk[i * 4 + 0] = o.x; pk[i * 4 + 1] = o.y; pk[i * 4 + 2] = o.z; pk[i * 4 + 3] = o.w;
+                    }
+                    tmem_st32u(tmem + lane_base + b * 64 + h * 32, pk);
                 }
-                fence_async_smem();
+                tmem_wait_st();
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_un(b));
             }
@@ -291,44 +314,59 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
         __syncwarp();
     } else if (warp == 9) {
         // =============================== MMA issuer ===============================
-        if (lane == 0) {
-            bool ok = true;
-            unsigned n_done = 0, n_acc = 0;   // blocks; accumulators handed over
-            int s = 0;
-            uint32_t phase = 0;               // of the slot's "full"
-            const uint32_t idesc = umma_idesc_mn(128, static_cast<uint32_t>(mt));
-            for (long long u = u0; ok && w4_segment(p, u, u0, u1, sg); u += sg.blocks) {
-                if (!kSmall)
-                    ok = mbar_wait(bar_acc_empty(static_cast<int>(n_acc & 1)), static_cast<uint32_t>(((n_acc >> 1) & 1) ^ 1), abort_word, p.status,
-                                   kWtWaitAccEmpty, p.wait_timeout_ns);
-                for (int j = 0; j < sg.blocks && ok; ++j, ++n_done) {
-                    const int b = static_cast<int>(n_done & 1);
-                    ok = mbar_wait(bar_in(s), phase, abort_word, p.status, kWtWaitIn, p.wait_timeout_ns) &&
-                         mbar_wait(bar_un(b), static_cast<uint32_t>((n_done >> 1) & 1), abort_word, p.status, kWtWaitUnpacked, p.wait_timeout_ns);
-                    if (ok && kSmall)
-                        ok = mbar_wait(bar_acc_empty(b), static_cast<uint32_t>(((n_done >> 1) & 1) ^ 1), abort_word, p.status, kWtWaitAccEmpty, p.wait_timeout_ns);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a_addr = s_un + b * kWtUnpacked, x_addr = s_in + s * stage_bytes;
+        // The whole warp walks the list, so that descriptors and addresses stay in uniform registers, and one elected
+        // lane issues.  A block's barriers are waited for side by side, a lane each (one after the other each costs about
+        // 100 clocks even when it is ready).  With one lane doing everything a block took 1100 clocks, whatever the rows.
+        bool ok = true;
+        unsigned n_done = 0, n_acc = 0;   // blocks; accumulators handed over
+        int s = 0;
+        uint32_t phase = 0;               // of the slot's "full"
+        const uint32_t idesc = umma_idesc_mn(128, static_cast<uint32_t>(mt));
+        for (long long u = u0; ok && w4_segment(p, u, u0, u1, sg); u += sg.blocks) {
+            for (int j = 0; j < sg.blocks && ok; ++j, ++n_done) {
+                const int b = static_cast<int>(n_done & 3), half = static_cast<int>(n_done & 1);
+                uint32_t bar = bar_in(s), par = phase;
+                int code = kWtWaitIn;
+                if (lane == 1) {
+                    bar = bar_un(b);
+                    par = (n_done >> 2) & 1u;
+                    code = kWtWaitUnpacked;
+                } else if (lane == 2 && kSmall) {
+                    bar = bar_acc_empty(half);
+                    par = ((n_done >> 1) & 1u) ^ 1u;
+                    code = kWtWaitAccEmpty;
+                } else if (lane == 2 && j == 0) {
+                    bar = bar_acc_empty(0);
+                    par = (n_acc & 1u) ^ 1u;
+                    code = kWtWaitAccEmpty;
+                }
+                ok = mbar_wait(bar, par, abort_word, p.status, code, p.wait_timeout_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t x_desc = umma_desc(s_in + s * stage_bytes, 0, 1024);   // (a step along K only adds to its address field)
+                const uint32_t x_half = static_cast<uint32_t>(mt * 128) >> 4;
+                if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t a_off = (ks >> 2) * (kWtUnpacked / 2) + (ks & 3) * 32, x_off = (ks >> 2) * mt * 128 + (ks & 3) * 32;
-                        const uint32_t d = kSmall ? tmem + (b * 4 + ks / (2 * kGW)) * mt : tmem + static_cast<uint32_t>(n_acc & 1) * 256;
+                        const uint32_t d = kSmall ? tmem + 256 + (half * 4 + ks / (2 * kGW)) * mt : tmem + 256;
                         const bool first = kSmall ? ks % (2 * kGW) == 0 : j == 0 && ks == 0;
-                        umma_bf16(d, umma_desc(a_addr + a_off, 0, 1024), umma_desc(x_addr + x_off, 0, 1024), idesc, !first);
+                        umma_bf16_a_tmem(d, tmem + b * 64 + ks * 8, x_desc + (ks >> 2) * x_half + (ks & 3) * 2, idesc, !first);
                     }
                     umma_commit(bar_un_empty(b));
                     umma_commit(bar_in_empty(s));
-                    if (kSmall) umma_commit(bar_acc(b));
-                    if (++s == p.stages) {
-                        s = 0;
-                        phase ^= 1;
-                    }
+                    if (kSmall) umma_commit(bar_acc(half));
+                    else if (j + 1 == sg.blocks) umma_commit(bar_acc(0));
                 }
-                if (!ok) break;
-                if (!kSmall) umma_commit(bar_acc(static_cast<int>(n_acc & 1)));
-                ++n_acc;
+                __syncwarp();
+                if (++s == p.stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
+            ++n_acc;
+        }
+        if (elect_one()) {
             umma_commit(bar_final);   // every MMA has completed before tensor memory is given back
             mbar_wait_quiet(bar_final, 0, *abort_word ? 2000000ull : p.wait_timeout_ns);
         }
@@ -346,16 +384,32 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                 if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
                 waited = true;
             };
-            auto store = [&](int m, float v) {   // column m of this weight row
-                if (sg.whole) {
-                    const int row = m0 + m;
-                    if (exists && row < p.m_rows && (row % p.max_batch) < p.batch) {
-                        if (p.residual) v += __bfloat162float(p.residual[row * p.ldr + n]);
-                        p.c[row * p.ldc + n] = __float2bfloat16_rn(v);
-                    }
-                } else {
-                    p.part[(static_cast<long long>(sg.slot) * mt + m) * kWtTileN + r] = v;
+            // rows m .. m + 15 of this weight row (the residual's values requested together)
+            const bool all_live = p.batch == p.max_batch;
+            auto store16 = [&](int m, float* v) {
+                if (!sg.whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p.part[(static_cast<long long>(sg.slot) * mt + m + i) * kWtTileN + r] = v[i];
+                    return;
                 }
+                unsigned live = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int row = m0 + m + i;
+                    if (exists && row < p.m_rows && (all_live || (row % p.max_batch) < p.batch)) live |= 1u << i;
+                }
+                if (p.residual) {
+                    __nv_bfloat16 res[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((live >> i) & 1u) res[i] = p.residual[(m0 + m + i) * p.ldr + n];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((live >> i) & 1u) v[i] += __bfloat162float(res[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if ((live >> i) & 1u) p.c[(m0 + m + i) * p.ldc + n] = __float2bfloat16_rn(v[i]);
             };
             if constexpr (kSmall) {
                 float acc[kMt];
@@ -382,7 +436,7 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
 #pragma unroll
                         for (int h = 0; h < kMt / 16; ++h) {
                             float v[16];
-                            tmem_ld16(tmem + lane_base + (b * 4 + g) * kMt + h * 16, v);
+                            tmem_ld16(tmem + lane_base + 256 + (b * 4 + g) * kMt + h * 16, v);
                             tmem_wait_ld();
 #pragma unroll
                             for (int m = 0; m < 16; ++m) acc[h * 16 + m] = fmaf(v[m], sc[g], acc[h * 16 + m]);
@@ -395,24 +449,22 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                 if (!ok) break;
                 before_store();
 #pragma unroll
-                for (int m = 0; m < kMt; ++m) store(m, acc[m]);
+                for (int m = 0; m < kMt; m += 16) store16(m, acc + m);
             } else {
-                const int b = static_cast<int>(n_acc & 1);
-                if (lane == 0) ok = mbar_wait(bar_acc(b), static_cast<uint32_t>((n_acc >> 1) & 1), abort_word, p.status, kWtWaitAcc, p.wait_timeout_ns);
+                if (lane == 0) ok = mbar_wait(bar_acc(0), n_acc & 1u, abort_word, p.status, kWtWaitAcc, p.wait_timeout_ns);
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                 if (!ok) break;
                 tc_fence_after();
                 before_store();
                 for (int m = 0; m < mt; m += 16) {
                     float v[16];
-                    tmem_ld16(tmem + lane_base + b * 256 + m, v);
+                    tmem_ld16(tmem + lane_base + 256 + m, v);
                     tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) store(m + i, v[i]);
+                    store16(m, v);
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_acc_empty(b));
+                if (lane == 0) mbar_arrive(bar_acc_empty(0));
                 ++n_acc;
             }
         }
