@@ -202,6 +202,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return mbar_wait_slow(bar, parity, abort_word, status, code, timeout_ns);
 }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
                                             int c2, int c3) {
     asm volatile(
@@ -1564,6 +1571,127 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             cp_async_wait<0>();   // (a wait that ran out: nothing of this warp's is in flight when the block ends)
         }
+    } else if (kExt != 0) {
+        // =============================== MMA issuer, kExt ===============================
+        // The same order of products as below.  The whole warp walks the list and one elected lane issues: addresses
+        // and descriptors then stay in uniform registers.  Issued by a lane of a divergent branch a product costs the
+        // issuing thread about 90 clocks, and the 32 of a step were what the step took.
+        if constexpr (kExt != 0) {
+            bool ok = true;
+            constexpr uint32_t idesc_qk = umma_idesc(false), idesc_pv = umma_idesc(true);
+            auto wait = [&](uint32_t bar, uint32_t par, int code) -> bool {
+                return __all_sync(0xffffffffu, mbar_wait(bar, par, abort_word, p.status, code, p.wait_timeout_ns)) != 0;
+            };
+            int slot_k = 0, slot_v = 0;              // ring slots of the next K and V tile to be used ...
+            int ring_slot = 0;                       // ... which follow one another in the ring
+            uint32_t ring_par = 0;
+            auto next_slot = [&]() {
+                if (++ring_slot == kTcStages) {
+                    ring_slot = 0;
+                    ring_par ^= 1;
+                }
+            };
+            unsigned steps_done[kTcTiles] = {0, 0}, q_loads[kTcTiles] = {0, 0}, tails = 0;
+            Item it;
+            for (long long k = 0; ok; ++k) {
+                int idx = n_items;
+                if (lane == 0) idx = take_item(k, ok, kTcWaitSched);
+                idx = __shfl_sync(0xffffffffu, idx, 0);
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(bar_sched_empty(static_cast<int>(k & 1)));
+                if (idx >= n_items) break;
+                tc_item(p, idx, it);
+                const int nsteps = it.nsteps;
+                auto wait_tile = [&](int item) -> bool {   // ring item `item` of this work item sits in ring_slot
+                    if (it.zero_tail && item == ((kExt & kExtBias) ? 1 : 2 * nsteps - 1))   // released by the producer's clean-up
+                        return wait(bar_tail, tails & 1u, kTcWaitKvFull);
+                    return wait(bar_kv_full(ring_slot), ring_par, kTcWaitKvFull);
+                };
+                auto issue_qk = [&](int t, int slot, bool last) {
+                    const uint64_t q_desc = umma_desc(smem_base + kTcSmemQ + t * kTcTileBytes, 0, 1024);
+                    const uint64_t k_desc = umma_desc(smem_base + kTcSmemRing + slot * kTcTileBytes, 0, 1024);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint32_t off = ((ks >> 2) * kTcHalfBytes + (ks & 3) * 32) >> 4;
+                            umma_bf16(tmem + t * 128, q_desc + off, k_desc + off, idesc_qk, ks > 0);
+                        }
+                        umma_commit(bar_s_full(t));
+                        if (!kSplit && last) umma_commit(bar_q_empty(t));   // this item reads Q_t no more
+                    }
+                    __syncwarp();
+                };
+                auto issue_pv = [&](int t, int slot, bool first) {
+                    const uint64_t v_desc = umma_desc(smem_base + kTcSmemRing + slot * kTcTileBytes, kTcHalfBytes, 1024);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            umma_bf16_a_tmem(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, v_desc + ((ks * 16 * 128) >> 4), idesc_pv, !(first && ks == 0));
+                        umma_commit(bar_pv_done(t));
+                    }
+                    __syncwarp();
+                };
+                for (int t = 0; t < kTcTiles && ok; ++t)
+                    if (it.steps[t] > 0) ok = wait(bar_q(t), q_loads[t] & 1u, kTcWaitQ);
+                if (ok && nsteps > 0) {
+                    ok = wait_tile(0);
+                    if (ok) {
+                        tc_fence_after();
+                        for (int t = 0; t < kTcTiles; ++t)
+                            if (it.steps[t] > 0) issue_qk(t, ring_slot, it.steps[t] == 1);
+                        if (elect_one()) umma_commit(bar_kv_empty(ring_slot));
+                        __syncwarp();
+                        next_slot();
+                    }
+                }
+                for (int j = 0; j < nsteps && ok; ++j) {
+                    bool have_v = false, have_k = false;
+                    for (int t = 0; t < kTcTiles && ok; ++t) {
+                        if (j >= it.steps[t]) continue;
+                        ok = wait(bar_p_full(t), (steps_done[t] + j) & 1u, kTcWaitPFull);
+                        if (!ok) break;
+                        if (!have_v) {
+                            ok = wait_tile(2 * j + 1);
+                            if (!ok) break;
+                            slot_v = ring_slot;
+                            next_slot();
+                            have_v = true;
+                        }
+                        tc_fence_after();
+                        issue_pv(t, slot_v, j == 0);
+                        if (j + 1 < it.steps[t]) {
+                            if (!have_k) {
+                                ok = wait_tile(2 * j + 2);
+                                if (!ok) break;
+                                slot_k = ring_slot;
+                                next_slot();
+                                have_k = true;
+                                tc_fence_after();
+                            }
+                            issue_qk(t, slot_k, j + 2 == it.steps[t]);
+                        }
+                    }
+                    if (!ok) break;
+                    if (elect_one()) {
+                        umma_commit(bar_kv_empty(slot_v));                      // V_j free once every MMA so far is done
+                        if (j + 1 < nsteps) umma_commit(bar_kv_empty(slot_k));  // and K_{j+1}
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (it.zero_tail && nsteps > 0) ++tails;
+                for (int t = 0; t < kTcTiles; ++t) {
+                    steps_done[t] += it.steps[t];
+                    if (it.steps[t] > 0) ++q_loads[t];
+                }
+            }
+            if (elect_one()) {
+                umma_commit(bar_final);   // every MMA issued above has completed before tensor memory is given back
+                mbar_wait_quiet(bar_final, 0, *abort_word ? 2000000ull : p.wait_timeout_ns);
+            }
+            __syncwarp();
+        }
     } else {
         // =============================== MMA issuer ===============================
         // One thread issues every MMA, one GEMM after the other: two issuing threads were tried and
@@ -1609,7 +1737,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // ring item i of this work item: K_(i/2) for even i, V_(i/2) for odd i
                 auto wait_item = [&](int item) {
                     const long long r = ring_c + item;
-                    if (it.zero_tail && item == ((kExt & kExtBias) ? 1 : 2 * nsteps - 1))   // this V tile is released by the producer's clean-up
+                    if (it.zero_tail && item == 2 * nsteps - 1)   // the last V tile is released by the producer's clean-up
                         return mbar_wait(bar_tail, static_cast<uint32_t>(tails & 1), abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
                     return mbar_wait(bar_kv_full(static_cast<int>(r % kTcStages)), static_cast<uint32_t>((r / kTcStages) & 1), abort_word,
                                      p.status, kTcWaitKvFull, p.wait_timeout_ns);
@@ -1624,7 +1752,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         for (int t = 0; t < kTcTiles; ++t)
                             if (it.steps[t] > 0) {
                                 issue_qk(t, slot_of(0));
-                                if (!kSplit && it.steps[t] == 1) umma_commit(bar_q_empty(t));   // this item reads Q_t no more
+                                if (it.steps[t] == 1) umma_commit(bar_q_empty(t));   // this item reads Q_t no more
                             }
                         umma_commit(bar_kv_empty(slot_of(0)));
                     }
@@ -1654,7 +1782,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                 tc_fence_after();
                             }
                             issue_qk(t, slot_k);
-                            if (!kSplit && j + 2 == it.steps[t]) umma_commit(bar_q_empty(t));
+                            if (j + 2 == it.steps[t]) umma_commit(bar_q_empty(t));
                         }
                     }
                     if (!ok) break;

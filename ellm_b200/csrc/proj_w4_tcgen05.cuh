@@ -77,13 +77,6 @@ __device__ __forceinline__ bool w4_segment(const W4TcParams& p, long long u, lon
     return true;
 }
 
-// True in one lane of the (converged) warp.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-
 // 8 weights of a word as four bf16 pairs in input order, (q - z) exactly, times s2 when kScale.  16 + q is the byte
 // 0x80 | q << 3 below the byte 0x41.
 template <bool kScale>
