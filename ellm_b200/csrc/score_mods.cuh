@@ -88,29 +88,49 @@ __device__ __noinline__ void exact_row(const ScoreMods m, const __nv_bfloat16* q
     float mx = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
     const long long own = hi > lo ? hi - lo : 0;
     const long long total = m.plen + own;
-    for (long long i = 0; i < total; ++i) {
-        const bool pre = i < m.plen;
-        const long long key = pre ? i : lo + (i - m.plen);
-        const uint2 uk = *reinterpret_cast<const uint2*>((pre ? pk + key * m.ps2 : k + key * s2) + lane * 4);
-        const uint2 uv = *reinterpret_cast<const uint2*>((pre ? pv + key * m.ps2 : v + key * s2) + lane * 4);
-        const float2 ka = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uk.x));
-        const float2 kb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uk.y));
-        const float2 va = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uv.x));
-        const float2 vb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uv.y));
-        float t = qf[0] * ka.x + qf[1] * ka.y + qf[2] * kb.x + qf[3] * kb.y;
+    constexpr int kN = 4;   // keys requested together: the walk's time is that of its loads
+    for (long long i = 0; i < total; i += kN) {
+        uint2 uk[kN], uv[kN];
+        float x[kN], p[kN];
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
-        const float x = mod_score(m, t, slope_log2, static_cast<float>(pos > key ? pos - key : key - pos));
-        const float m_new = fmaxf(mx, x);
+        for (int n = 0; n < kN; ++n) {
+            const long long at = min(i + n, total - 1);
+            const bool pre = at < m.plen;
+            const long long key = pre ? at : lo + (at - m.plen);
+            uk[n] = *reinterpret_cast<const uint2*>((pre ? pk + key * m.ps2 : k + key * s2) + lane * 4);
+            uv[n] = *reinterpret_cast<const uint2*>((pre ? pv + key * m.ps2 : v + key * s2) + lane * 4);
+            if (i + n >= total) uv[n] = make_uint2(0u, 0u);
+            x[n] = static_cast<float>(pos > key ? pos - key : key - pos);
+        }
+        float m_new = mx;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const float2 ka = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uk[n].x));
+            const float2 kb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uk[n].y));
+            float t = qf[0] * ka.x + qf[1] * ka.y + qf[2] * kb.x + qf[3] * kb.y;
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+            x[n] = i + n < total ? mod_score(m, t, slope_log2, x[n]) : -INFINITY;
+            m_new = fmaxf(m_new, x[n]);
+        }
         const float msub = m_new == -INFINITY ? 0.0f : m_new;
-        const float corr = fast_exp2(mx - msub), p = fast_exp2(x - msub);
+        const float corr = fast_exp2(mx - msub);
         mx = m_new;
-        l = l * corr + p;
-        o[0] = o[0] * corr + p * va.x;
-        o[1] = o[1] * corr + p * va.y;
-        o[2] = o[2] * corr + p * vb.x;
-        o[3] = o[3] * corr + p * vb.y;
-        if ((i & 63) == 63 && __all_sync(0xffffffffu, isnan(l) && isnan(o[0]) && isnan(o[1]) && isnan(o[2]) && isnan(o[3]))) break;
+        l *= corr;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] *= corr;
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const float2 va = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uv[n].x));
+            const float2 vb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uv[n].y));
+            p[n] = fast_exp2(x[n] - msub);
+            l += p[n];
+            o[0] += p[n] * va.x;
+            o[1] += p[n] * va.y;
+            o[2] += p[n] * vb.x;
+            o[3] += p[n] * vb.y;
+        }
+        if ((i & 63) == 60 && __all_sync(0xffffffffu, isnan(l) && isnan(o[0]) && isnan(o[1]) && isnan(o[2]) && isnan(o[3]))) break;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint2 r;
