@@ -163,7 +163,7 @@ struct ellm_attn {
     bool scores_on = false, prefix_on = false;
     float* pre_part = nullptr;         // shared prefix, decode steps: partial O [pre_slots][128], then partial LSE [pre_slots]
     size_t pre_slots = 0;
-    double prefix_flat_flops = 1.2e9;  // see prefix_is_flat
+    long long prefix_flat_keys = 55000;   // see prefix_is_flat
     std::mutex mu;
     uint64_t launches[ELLM_KERNEL_COUNT] = {};
     uint64_t timed[ELLM_KERNEL_COUNT] = {};
@@ -303,11 +303,16 @@ cudaError_t launch_merge(const ellm::DecodeParams& p, size_t batch, unsigned blo
                  : cudaLaunchKernelEx(&cfg, ellm::decode_merge_kernel<__nv_bfloat16, 8, 10>, p, ob, lse_out, pieces_cap);
 }
 
-// Whether a decode step takes its shared prefix in the split-KV kernel's own tile list (one launch less, the
-// prefix read once per 16 query rows, warp-level products) or in the tensor-memory kernel (once per 256 rows, a
-// launch and a start-up of about 12 us more).  By the prefix's FLOPs.
+// Whether a decode step takes its shared prefix in the split-KV kernel's own tile list or in the tensor-memory kernel
+// ahead of it.  The former is one launch less (about 8.5 us for short prefixes) and reads the prefix once per 16 query
+// rows of a KV head, each time for about 0.1 us per 1000 (key, KV head); the latter starts at 15 us and takes 0.14 us
+// per 1000, up to 256 query rows at once.  Split-KV / tensor-memory kernel, us, at (q heads, kv heads) (32, 4), 16-row
+// blocks b and keys x KV heads in thousands: 1 block of 262: 36 / 55; 2 of 66: 27.5 / 27; 4 of 16: 19.5 / 19.8, of 66: 33 / 28;
+// 8 of 4: 15.6 / 17.5, of 16: 32 / 23; 16 of 4: 23.5 / 23.7, of 262: 500 / 70; 32 of 4: 38 / 28, of 66: 277 / 51.
 bool prefix_is_flat(const ellm_attn* h, size_t batch) {
-    return !h->tc.ready_ext || 4.0 * ellm::kHeadDim * static_cast<double>(h->mods.plen) * static_cast<double>(batch * h->d.q_heads) < h->prefix_flat_flops;
+    if (!h->tc.ready_ext) return true;
+    const double rows = static_cast<double>(batch * h->group), extra = std::ceil(rows / 16.0) - 1.4 * std::ceil(rows / 256.0);
+    return h->prefix_flat_keys > 0 && static_cast<double>(h->mods.plen) * static_cast<double>(h->d.kv_heads) * extra < static_cast<double>(h->prefix_flat_keys);
 }
 size_t prefix_flat_slots(const ellm_attn* h) {
     return h->slots + h->d.kv_heads * ((h->d.max_batch * h->group + 15) / 16);
@@ -1327,9 +1332,9 @@ int ellm_attn_set_option(ellm_attn* h, const char* name, long long value) {
         h->decode_early = value != 0;
         return ELLM_OK;
     }
-    if (std::strcmp(name, "prefix_flat_mflops") == 0) {
-        if (value < 0) return fail(ELLM_ERR_INVALID_ARG, "prefix_flat_mflops must be >= 0");
-        h->prefix_flat_flops = static_cast<double>(value) * 1e6;
+    if (std::strcmp(name, "prefix_flat_keys") == 0) {
+        if (value < 0) return fail(ELLM_ERR_INVALID_ARG, "prefix_flat_keys must be >= 0");
+        h->prefix_flat_keys = value;
         return ELLM_OK;
     }
     if (std::strcmp(name, "tc_fuse_append") == 0) {

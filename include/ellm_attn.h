@@ -369,7 +369,8 @@ int ellm_attn_decode_noalloc(const void* q, const void* k_cache, const void* v_c
  *                           rows before it waits for the stream's previous kernel, so that its start
  *                           overlaps that kernel's end.  The caller vouches that the previous kernel in
  *                           the stream writes neither the positions nor cache rows below each sequence's
- *                           newest row, and (if it is not one of this library's) that it was itself
+ *                           newest row, nor the arrays of ellm_attn_set_scores, nor the shared prefix's
+ *                           rows, and (if it is not one of this library's) that it was itself
  *                           ordered after whatever does.  True for the decode steps of a layer stack -
  *                           the projection before attention writes only Q and the newest row - and for
  *                           back-to-back steps on resident inputs; default 0.  ellm_attn_run_host never
@@ -380,9 +381,9 @@ int ellm_attn_decode_noalloc(const void* q, const void* k_cache, const void* v_c
  *                           first.  Same cache bits either way.
  *   "tc_persistent"         prefill kernel: -1 (default) / 1 one CTA per SM walking the work-item list,
  *                           0 one CTA per item; a tuning knob.
- *   "prefix_flat_mflops"    decode steps with a shared prefix: below this many MFLOP (4 x 128 x prefix_len x batch x
- *                           query heads) the prefix goes through the split-KV kernel, from there on through the
- *                           tensor-memory kernel; a tuning knob (0: always the latter).
+ *   "prefix_flat_keys"      decode steps with a shared prefix: how many keys x KV heads the split-KV kernel may read
+ *                           for blocks of 16 query rows beyond what the tensor-memory kernel would (default 55000);
+ *                           above it the prefix goes through the latter.  A tuning knob (0: always the latter).
  *   "decode_ctas"           grid of the decode kernel, 1 .. 2 x SMs (default 2 x SMs, for which the
  *                           workspace is sized); a tuning knob.
  * Unknown names return ELLM_ERR_INVALID_ARG.  The reference has no counterpart (it aborts). */
