@@ -133,6 +133,12 @@ class Attention {
                     size_t thread_id) const {
         check(ellm_attn_run_ragged(handle_, positions, position_interval, batch_size, cpu_num, thread_id));
     }
+    // Extensions: modified scores and a shared prefix for the runs that follow (ellm_attn_set_scores,
+    // ellm_attn_set_shared_prefix); a default-constructed ellm_attn_scores / a null k takes them off.
+    void set_scores(const ellm_attn_scores& scores) const { check(ellm_attn_set_scores(handle_, &scores)); }
+    void set_shared_prefix(const T* k, const T* v, size_t kv_head_stride, size_t position_stride, size_t prefix_len) const {
+        check(ellm_attn_set_shared_prefix(handle_, k, v, kv_head_stride, position_stride, prefix_len));
+    }
     // For async operators: waits for the stream and throws if a device-side wait ran out since the last check.
     void check_device() const { check(ellm_attn_check(handle_)); }
 
@@ -269,6 +275,51 @@ class MatMulAdd {
   private:
     MatMulAdd() = default;
     ellm_matmul_add* handle_ = nullptr;
+};
+
+// output = residual + A . W^T with 4-bit weights W[n][k] = (q[n][k] - z) * scale, one scale (and zero point) per
+// `group` inputs (ellm_matmul_add_w4_desc has the layouts); zeros null = 8 everywhere.
+template <typename T>
+class MatMulAddW4 {
+    static_assert(sizeof(T) == 2, "bf16 storage (2-byte elements) only");
+
+  public:
+    static MatMulAddW4 make(const T* ptr1, const uint8_t* w4, const T* scales, const uint8_t* zeros, size_t group, const T* ptr3,
+                            T* output_ptr, size_t m_max, size_t n_max, size_t k_max, const ProjectionOptions& opt) {
+        ellm_matmul_add_w4_desc d{};
+        d.a = ptr1;
+        d.w4 = w4;
+        d.scales = scales;
+        d.zeros = zeros;
+        d.group = group;
+        d.residual = ptr3;
+        d.output = output_ptr;
+        d.m_max = m_max;
+        d.n_max = n_max;
+        d.k_max = k_max;
+        d.max_batch = opt.max_batch;
+        d.device = opt.device;
+        d.stream = opt.stream;
+        d.async = opt.async ? 1 : 0;
+        MatMulAddW4 m;
+        check(ellm_matmul_add_w4_create(&d, &m.handle_));
+        return m;
+    }
+    MatMulAddW4(MatMulAddW4&& o) noexcept : handle_(o.handle_) { o.handle_ = nullptr; }
+    MatMulAddW4(const MatMulAddW4&) = delete;
+    MatMulAddW4& operator=(const MatMulAddW4&) = delete;
+    ~MatMulAddW4() { ellm_matmul_add_w4_destroy(handle_); }
+    void run(size_t position_index, size_t position_interval, size_t batch_size, size_t cpu_num, size_t thread_id) const {
+        check(ellm_matmul_add_w4_run(handle_, position_index, position_interval, batch_size, cpu_num, thread_id));
+    }
+    void run_ragged(const int32_t*, size_t position_interval, size_t batch_size, size_t cpu_num, size_t thread_id) const {
+        run(0, position_interval, batch_size, cpu_num, thread_id);
+    }
+    void check_device() const { check(ellm_matmul_check(handle_, 2)); }
+
+  private:
+    MatMulAddW4() = default;
+    ellm_matmul_add_w4* handle_ = nullptr;
 };
 
 // One entry of the executor's operator queue: any operator behind the common run() signature

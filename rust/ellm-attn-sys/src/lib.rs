@@ -100,10 +100,42 @@ pub struct ellm_matmul_add_desc {
     pub r#async: c_int,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ellm_matmul_add_w4_desc {
+    pub a: *const c_void,
+    pub a_row_stride: usize,
+    pub w4: *const c_void,
+    pub scales: *const c_void,
+    pub zeros: *const c_void,
+    pub group: usize,
+    pub residual: *const c_void,
+    pub residual_row_stride: usize,
+    pub output: *mut c_void,
+    pub output_row_stride: usize,
+    pub m_max: usize,
+    pub n_max: usize,
+    pub k_max: usize,
+    pub max_batch: usize,
+    pub device: c_int,
+    pub stream: *mut c_void,
+    pub r#async: c_int,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ellm_attn_scores {
+    pub softcap: f32,
+    pub slopes: *const f32,
+    pub row_begin: *const i32,
+    pub row_begin_stride: usize,
+    pub prefix_lens: *const i32,
+}
+
 macro_rules! opaque {
     ($($name:ident),*) => { $( #[repr(C)] pub struct $name { _private: [u8; 0] } )* };
 }
-opaque!(ellm_attn, ellm_matmul3, ellm_matmul_add, ellm_kv_cache, ellm_step_graph);
+opaque!(ellm_attn, ellm_matmul3, ellm_matmul_add, ellm_matmul_add_w4, ellm_kv_cache, ellm_step_graph);
 
 #[link(name = "ellm_attn")]
 extern "C" {
@@ -124,6 +156,9 @@ extern "C" {
     pub fn ellm_attn_run_window_q(h: *mut ellm_attn, q: *const c_void, position_index: usize,
                                   position_interval: usize, batch_size: usize, key_begin: usize,
                                   key_end: usize, o_part: *mut f32, lse_part: *mut f32) -> c_int;
+    pub fn ellm_attn_set_scores(h: *mut ellm_attn, s: *const ellm_attn_scores) -> c_int;
+    pub fn ellm_attn_set_shared_prefix(h: *mut ellm_attn, k: *const c_void, v: *const c_void, kv_head_stride: usize,
+                                       position_stride: usize, prefix_len: usize) -> c_int;
     pub fn ellm_attn_check(h: *mut ellm_attn) -> c_int;
     pub fn ellm_attn_set_option(h: *mut ellm_attn, name: *const c_char, value: c_longlong) -> c_int;
     pub fn ellm_attn_set_profiling(h: *mut ellm_attn, on: c_int) -> c_int;
@@ -179,6 +214,10 @@ extern "C" {
     pub fn ellm_matmul_add_destroy(h: *mut ellm_matmul_add) -> c_int;
     pub fn ellm_matmul_add_run(h: *mut ellm_matmul_add, position_index: usize, position_interval: usize,
                                batch_size: usize, cpu_num: usize, thread_id: usize) -> c_int;
+    pub fn ellm_matmul_add_w4_create(desc: *const ellm_matmul_add_w4_desc, out: *mut *mut ellm_matmul_add_w4) -> c_int;
+    pub fn ellm_matmul_add_w4_destroy(h: *mut ellm_matmul_add_w4) -> c_int;
+    pub fn ellm_matmul_add_w4_run(h: *mut ellm_matmul_add_w4, position_index: usize, position_interval: usize,
+                                  batch_size: usize, cpu_num: usize, thread_id: usize) -> c_int;
     pub fn ellm_matmul_set_profiling(handle: *mut c_void, which: c_int, on: c_int) -> c_int;
     pub fn ellm_matmul_kernel_stats(handle: *mut c_void, which: c_int, launches: *mut u64,
                                     timed_launches: *mut u64, ms: *mut f64) -> c_int;
