@@ -21,12 +21,16 @@ def _ptr(x):
     return x.data_ptr()
 
 
-def _check_tensor(name, t, dtype, shape):
+def _on_device(t, device):
+    return t.is_cuda and t.device.index == device
+
+
+def _check_tensor(name, t, dtype, shape, device):
     """A torch tensor handed over as a device array: its type, size and place (raw pointers pass)."""
     if t is None or not hasattr(t, "data_ptr"):
         return
-    if str(t.dtype) != "torch." + dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor of shape {list(shape)}")
+    if str(t.dtype) != "torch." + dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not _on_device(t, device):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on CUDA device {device}")
 
 
 class Attention:
@@ -119,15 +123,15 @@ class Attention:
         positions every row of the sequence sees.  Tensors are device buffers read by every run; without any
         argument the operator goes back to plain attention."""
         d = self.desc
-        _check_tensor("slopes", slopes, "float32", (d.q_heads,))
-        _check_tensor("prefix_lens", prefix_lens, "int32", (d.max_batch,))
+        _check_tensor("slopes", slopes, "float32", (d.q_heads,), d.device)
+        _check_tensor("prefix_lens", prefix_lens, "int32", (d.max_batch,), d.device)
         stride = d.max_seq
         if hasattr(row_begin, "data_ptr"):
             if str(row_begin.dtype) != "torch.int32" or row_begin.dim() != 2 or row_begin.shape[0] < d.max_batch \
                     or row_begin.shape[1] < d.max_seq or row_begin.stride(1) != 1:
                 raise ValueError(f"row_begin must be int32 [{d.max_batch}, >= {d.max_seq}] with contiguous rows")
-            if not row_begin.is_cuda:
-                raise ValueError("row_begin must be a CUDA tensor")
+            if not _on_device(row_begin, d.device):
+                raise ValueError(f"row_begin must be on CUDA device {d.device}")
             # (the stride of a one-row tensor says nothing)
             stride = row_begin.stride(0) if row_begin.shape[0] > 1 else row_begin.shape[1]
         s = L.AttnScores(float(softcap), _ptr(slopes), _ptr(row_begin), stride, _ptr(prefix_lens))
@@ -145,10 +149,10 @@ class Attention:
             return
         if hasattr(k, "data_ptr"):
             for name, t in (("k", k), ("v", v)):
-                if str(t.dtype) != "torch.bfloat16" or not t.is_cuda or t.dim() != 3 or t.stride(2) != 1 \
+                if str(t.dtype) != "torch.bfloat16" or not _on_device(t, self.desc.device) or t.dim() != 3 or t.stride(2) != 1 \
                         or t.shape[0] < self.desc.kv_heads or t.shape[2] != self.desc.head_size:
-                    raise ValueError(f"{name} must be a bf16 CUDA tensor [{self.desc.kv_heads}, rows, {self.desc.head_size}] "
-                                     "with contiguous rows")
+                    raise ValueError(f"{name} must be bf16 [{self.desc.kv_heads}, rows, {self.desc.head_size}] with contiguous "
+                                     f"rows on CUDA device {self.desc.device}")
             if k.shape != v.shape or k.stride() != v.stride():
                 raise ValueError("k and v must have the same shape and strides")
             if prefix_len is None:

@@ -143,7 +143,7 @@ class MatMulAddW4(_Projection):
         lib = L.load()
         for name, t, dtype, width in (("w4_ptr", w4_ptr, "uint8", k_max // 2), ("scales_ptr", scales_ptr, "bfloat16", k_max // max(group, 1)),
                                       ("zeros", zeros, "uint8", k_max // max(group, 1))):
-            _check_tensor(name, t, dtype, (n_max, width))
+            _check_tensor(name, t, dtype, (n_max, width), device)
         d = L.MatMulAddW4Desc()
         d.a, d.a_row_stride, d.w4 = _ptr(ptr1), a_row_stride, _ptr(w4_ptr)
         d.scales, d.zeros, d.group = _ptr(scales_ptr), _ptr(zeros), group
