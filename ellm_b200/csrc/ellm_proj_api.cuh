@@ -522,8 +522,6 @@ W4Choice w4_choice_of(size_t group) {
                           : ellm::proj_w4_kernel<CB, WN, NB, 1>,
             ellm::W4Shape<CB, WN, NB>::kThreads, ellm::W4Shape<CB, WN, NB>::kSmemBytes};
 }
-// Warps across the columns and blocks per warp by the blocks a CTA has: one block leaves all 16 warps to K,
-// four and more put four warps across (a chunk of the rows then serves up to 16 blocks).
 // The tensor-memory form for `rows` per tile: exact up to 32, weights rounded to bf16 above.
 typedef void (*W4TcKernel)(const CUtensorMap, const uint8_t*, const ellm::W4TcParams);
 template <bool kSmall, int kMt>
@@ -535,6 +533,8 @@ W4TcKernel w4_tc_kernel(int mt, size_t group) {
     return mt == 16 ? w4_tc_kernel_of<true, 16>(group) : mt == 32 ? w4_tc_kernel_of<true, 32>(group) : w4_tc_kernel_of<false, 0>(group);
 }
 
+// Warps across the columns and blocks per warp by the 16-column blocks a CTA has: one block leaves all 16 warps to K,
+// four and more put four warps across (a chunk of the rows then serves up to 16 blocks).
 template <int NB>
 W4Choice w4_choice(size_t n, size_t group, int sm_count) {
     const size_t blocks = ((n + 15) / 16 + sm_count - 1) / sm_count;

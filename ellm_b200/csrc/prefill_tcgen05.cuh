@@ -31,16 +31,25 @@
 // kExt instantiations (score_mods.cuh): scores capped and biased, a key interval per row, key tiles of a
 // shared prefix ahead of the sequence's own, and any group of up to 128 query heads (a row tile holds the
 // floor(128 / G) positions that fit).  An item walks the 128-key tiles from the first to the last key any of
-// its rows sees; tiles that all rows of a row tile see whole take the one-pass step, the others the two-pass
-// step with the interval applied.  The interval hulls come from a table filled by a small kernel ahead
+// its rows sees; a tile that some row of a row tile does not see whole is exponentiated under per-row bit masks,
+// in the same one-pass step.  The interval hulls come from a table filled by a small kernel ahead
 // of this one (row_begin), or follow from the positions alone.
+// What bounds it: the softmax warps.  A 128-key step of both row tiles takes about 3700 clocks plain, 5000 capped
+// (five multiply-adds a score for the tanh) and 4300 biased, against 2800 for its products; an item costs about
+// 11000 clocks besides its steps (queries, first tile, epilogue), which is what short documents and windows pay.
+// Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.55 ms (862 TFLOP/s); 2 x 8191 tokens of
+// documents of about 900, biased, 32 / 8 heads, 365 us; 8 x 256 rows under a capped 1024-key window, 64 / 8 heads, 140 us;
+// 16 x 48 rows after 8190 shared keys, 32 / 4 heads, 160 us (646 TFLOP/s).
 //
 // kExtSplit: the shared-prefix part of a decode step.  The rows are the step's query rows (chunk row =
 // sequence), the keys the prefix alone, cut into `splits` runs of tiles so that every SM has work, and the
 // result is one fp32 partial (O, LSE) per run; the sequences' own keys go through the split-KV kernel and its
 // merge takes these partials in.  The prefix is read once per 256 query rows of a KV head instead of once per
-// sequence.  A K/V tile is used by one or two CTAs only, so the tiles come from HBM, where one TMA queue per SM
-// brings no more than about 20 GB/s: two further warps load them with 16-byte asynchronous copies instead.
+// sequence.  A K/V tile is used by one or two CTAs only and comes from HBM: two further warps load the tiles with
+// 16-byte asynchronous copies instead of the TMA producer (64 sequences of 32 / 4 heads on 32768 keys: 99 -> 94 us
+// when that was introduced).  That step takes 81 us now, 134 MB of prefix and own keys: not the stream but the chain of
+// a step (4000 to 5000 clocks), 10000 clocks to the first tile and 4000 of epilogue bound it - the same step on a
+// prefix that stays in L2 takes as long.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>

@@ -122,10 +122,15 @@ int ellm_matmul_add_run(ellm_matmul_add* h, size_t position_index, size_t positi
 /* ---- MatMulAddW4: output = residual + A . W^T with 4-bit weights --------------------------------
  * MatMulAdd for a checkpoint whose weights are 4-bit numbers with one scale per group of inputs:
  *     W[n][k] = (q[n][k] - z[n][k / group]) * scale[n][k / group],   q in 0..15.
- * The sum is formed in fp32 and rounded to bf16 once; runs of at most 16 rows multiply by q - z and
+ * The sum is formed in fp32 and rounded to bf16 once; runs of at most 32 rows multiply by q - z and
  * apply the scale to the fp32 sums, larger ones multiply by W rounded to bf16.  Weights, scales and
- * zero points are read by every run, in place; a handle for more than 16 rows keeps a bf16 workspace
- * of n_max x k_max.  Handles of this kind are `which` 2 of the ellm_matmul_* calls below. */
+ * zero points are read by every run, in place, and (like the weights of the other projections in a decode
+ * step) ahead of the wait for the stream's previous kernel: after a kernel that rewrites them, wait for the
+ * stream before the next run.  A handle keeps 2 x SMs x min(256, m_max) x 128 fp32 of workspace, so runs of
+ * one handle must not overlap.  Rows hold finite numbers (a row with an infinity may come out as NaN where
+ * the plain sum is infinite); rows with (row % max_batch) >= batch_size reach no result and are not written.
+ * Handles of this kind are `which` 2 of the ellm_matmul_* calls below.  No counterpart in the reference,
+ * whose weights have the activations' type (src/compiler/mul/matmul_add.rs:60-126). */
 typedef struct ellm_matmul_add_w4 ellm_matmul_add_w4;
 
 typedef struct ellm_matmul_add_w4_desc {
