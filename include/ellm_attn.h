@@ -369,12 +369,12 @@ int ellm_attn_decode_noalloc(const void* q, const void* k_cache, const void* v_c
  *                           rows before it waits for the stream's previous kernel, so that its start
  *                           overlaps that kernel's end.  The caller vouches that the previous kernel in
  *                           the stream writes neither the positions nor cache rows below each sequence's
- *                           newest row, nor the arrays of ellm_attn_set_scores, nor the shared prefix's
- *                           rows, and (if it is not one of this library's) that it was itself
+ *                           newest row, and (if it is not one of this library's) that it was itself
  *                           ordered after whatever does.  True for the decode steps of a layer stack -
  *                           the projection before attention writes only Q and the newest row - and for
  *                           back-to-back steps on resident inputs; default 0.  ellm_attn_run_host never
- *                           uses it (its staging kernel writes the positions).
+ *                           uses it (its staging kernel writes the positions), nor do steps with
+ *                           modified scores or a shared prefix.
  *   "tc_fuse_append"        prefill kernel: 1 (default) the chunk's K/V rows are read from k_new / v_new and
  *                           written into the cache by the attention kernel itself when the chunk starts on a
  *                           128-key boundary (one start for all sequences); 0 always runs the append kernel
