@@ -4,13 +4,15 @@
 //     its N side (16 to 256), so that a handful of rows costs the tensor unit a handful of columns.
 //
 // What bounds it: up to 32 rows it should be the packed weights from HBM (0.5 byte each), with a prompt chunk the
-// products.  What does today is between the two, the unpacking: about 14 instructions per 8 weights, done once per weight
-// and row tile, and the hand-over of a block from unpackers to products to drain.  Measured: 13 x 28672 x 8192 56 us
-// (117 MB of weights, 2.1 TB/s), 600 x 8192 x 8192 113 us (713 TFLOP/s), of which the reduction is about 10.
+// products.  What does today is the chain of the warp that issues them: about 1200 clocks for a 128-input block
+// whatever the rows (its barriers, the products' issue, the commits), against 100 (16 rows) to 830 (208 rows) of
+// products; the unpackers, about 14 instructions per 8 weights, wait for a free buffer more than half of the time.
+// Measured: 13 x 28672 x 8192 59 us (117 MB of weights, 2.0 TB/s), 600 x 8192 x 8192 104 to 113 us by what L2 holds
+// (713 TFLOP/s at 113).
 //   warps 0-7   unpack: two groups of four, one block each in turn; a thread has one weight row.  A warp streams its
 //               32 rows' packed words through a private ring of 16-byte asynchronous copies and stores the bf16 pairs
 //               into tensor memory, where the MMA takes its A operand from: no shared-memory round trip and no proxy
-//               fence (600 x 8192 x 8192: 122 us through shared memory, 113 so)
+//               fence (through shared memory, three buffers: 13 x 28672 x 8192 64 -> 76 us, 600 x 8192 x 8192 104 -> 109)
 //   warp  8     TMA producer of the rows (m x 256 bytes per 128-input block)
 //   warp  9     MMA issuer, owner of tensor memory
 //   warps 10-13 drain / epilogue: thread = one weight row
