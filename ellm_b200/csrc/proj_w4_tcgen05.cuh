@@ -7,8 +7,8 @@
 // products.  What does today is the chain of the warp that issues them: about 1200 clocks for a 128-input block
 // whatever the rows (its barriers, the products' issue, the commits), against 100 (16 rows) to 830 (208 rows) of
 // products; the unpackers, about 14 instructions per 8 weights, wait for a free buffer more than half of the time.
-// Measured: 13 x 28672 x 8192 59 us (117 MB of weights, 2.0 TB/s), 600 x 8192 x 8192 104 to 113 us by what L2 holds
-// (713 TFLOP/s at 113).
+// Measured: 13 x 28672 x 8192 59 us (117 MB of weights, 2.0 TB/s), 600 x 8192 x 8192 100 to 110 us by what L2 holds
+// (731 TFLOP/s at 110).
 //   warps 0-7   unpack: two groups of four, one block each in turn; a thread has one weight row.  A warp streams its
 //               32 rows' packed words through a private ring of 16-byte asynchronous copies and stores the bf16 pairs
 //               into tensor memory, where the MMA takes its A operand from: no shared-memory round trip and no proxy
@@ -322,21 +322,13 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
         for (long long u = u0; ok && w4_segment(p, u, u0, u1, sg); u += sg.blocks) {
             for (int j = 0; j < sg.blocks && ok; ++j, ++n_done) {
                 const int b = static_cast<int>(n_done & 3), half = static_cast<int>(n_done & 1);
-                uint32_t bar = bar_in(s), par = phase;
-                int code = kWtWaitIn;
-                if (lane == 1) {
-                    bar = bar_un(b);
-                    par = (n_done >> 2) & 1u;
-                    code = kWtWaitUnpacked;
-                } else if (lane == 2 && kSmall) {
-                    bar = bar_acc_empty(half);
-                    par = ((n_done >> 1) & 1u) ^ 1u;
-                    code = kWtWaitAccEmpty;
-                } else if (lane == 2 && j == 0) {
-                    bar = bar_acc_empty(0);
-                    par = (n_acc & 1u) ^ 1u;
-                    code = kWtWaitAccEmpty;
-                }
+                // (chosen without branches: three divergent ones cost 4 % of a chunk)
+                const uint32_t acc_bar = kSmall ? bar_acc_empty(half) : bar_acc_empty(0);
+                const uint32_t acc_par = (kSmall ? (n_done >> 1) & 1u : n_acc & 1u) ^ 1u;
+                const bool on_acc = lane == 2 && (kSmall || j == 0);
+                const uint32_t bar = lane == 1 ? bar_un(b) : on_acc ? acc_bar : bar_in(s);
+                const uint32_t par = lane == 1 ? (n_done >> 2) & 1u : on_acc ? acc_par : phase;
+                const int code = lane == 1 ? kWtWaitUnpacked : on_acc ? kWtWaitAccEmpty : kWtWaitIn;
                 ok = mbar_wait(bar, par, abort_word, p.status, code, p.wait_timeout_ns);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
