@@ -16,13 +16,12 @@
 //     32-block, so no product mixes two groups and the scale is applied to the fp32 sums, not to the
 //     weights.
 //   * Unpacking decides the rate (every weight is unpacked once per step): a word becomes four bf16 pairs
-//     with a shift and a logic operation each.  What the tensor core multiplies is 16 + q, exact in bf16; a
-//     group's sum starts at -(16 + z) * (sum of the row's inputs over the group), so it ends at the sum over
-//     (q - z) * x.  The sums on the way are up to (16 + z) sum |x|, so their fp32 roundings (2^-24 each) are a
-//     few 1e-6 of sum |x| |q - z|, far below the output's 2^-8.
+//     128 + q with a logic operation each (and a shift for three of them), from which a packed subtraction takes
+//     128 + z.  Both and their difference q - z are exact in bf16, so the tensor core multiplies q - z itself: a weight
+//     of zero adds nothing, and the roundings are those of the sum's own terms.
 // The sums of the WK warps of a column are added in warp order: the result does not depend on timing.
-// Measured: 1 x 2048 x 4096 3.9 us (a launch and two round trips to memory for 4 MB), 8 x 8192 x 8192 20 us,
-// 8 x 28672 x 8192 58 us (2.0 TB/s: unpacking and products bound it, not the stream).
+// Measured, groups of 128: 1 x 2048 x 4096 3.9 us (a launch and two round trips to memory for 4 MB), 8 x 8192 x 8192
+// 19.4 us (1.8 TB/s: unpacking and products bound it, not the stream; groups of 32 21.0 us).
 //
 // Large weights and more rows: proj_w4_tcgen05.cuh.
 #pragma once
@@ -68,16 +67,20 @@ struct W4Shape {
     __device__ static constexpr int swz(int r) { return kKB == 2 ? (r & 7) : ((r >> 1) & 3); }
 };
 
-// The numbers of inputs (i, i + 4), i = 0..3, of a word of 8, as bf16 pairs of 16 + q (exact: 0x4180 is 16,
-// q its four leading mantissa bits).
-__device__ __forceinline__ void w4_pairs(uint32_t word, uint32_t sixteens, uint32_t (&r)[4]) {
-    const uint32_t s[4] = {word << 3, word >> 1, word >> 5, word >> 9};
+// q - z of inputs (i, i + 4), i = 0..3, of a word of 8, as bf16 pairs.  128 + q and 128 + z (z up to 127, `zero` holds it
+// twice) are the bf16 numbers 0x4300 | q and 0x4300 | z.
+__device__ __forceinline__ void w4_pairs(uint32_t word, uint32_t base, uint32_t zero, uint32_t (&r)[4]) {
+    const uint32_t s[4] = {word, word >> 4, word >> 8, word >> 12};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) asm("lop3.b32 %0, %1, 0x00780078, %2, 0xea;" : "=r"(r[i]) : "r"(s[i]), "r"(sixteens));   // (s & mask) | 16
+    for (int i = 0; i < 4; ++i) {
+        asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(r[i]) : "r"(s[i]), "r"(base));   // (s & mask) | base
+        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&r[i]), *reinterpret_cast<const __nv_bfloat162*>(&zero));
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
 }
-// -(16 + z), z (up to 127) being byte `gr` of four
-__device__ __forceinline__ float w4_minus_zero(uint32_t z4, int gr) {
-    return 112.0f - __uint_as_float(__byte_perm(z4, 0x43000000u, 0x7044u + (static_cast<uint32_t>(gr) << 8)));   // 0x43zz0000 = 128 + z
+// 128 + z twice, z being byte `gr` of four
+__device__ __forceinline__ uint32_t w4_zero_pair(uint32_t z4, int gr) {
+    return __byte_perm(z4, 0x43434343u, 0x4040u + 0x0101u * static_cast<uint32_t>(gr));
 }
 
 template <int CB, int WN, int NB, int GW>   // GW: 32-blocks per group (group = 32 * GW)
@@ -101,8 +104,8 @@ __global__ void __launch_bounds__(W4Shape<CB, WN, NB>::kThreads, 1) proj_w4_kern
     const long long row_bytes = p.k / 2;
     const int groups_row = p.k / (32 * GW), blocks_k = p.k / 128;
     bool waited = false;
-    uint32_t sixteens;
-    asm volatile("mov.u32 %0, 0x41804180;" : "=r"(sixteens));   // (opaque: kept in a register, so that w4_pairs is one operation per pair)
+    uint32_t base;
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(base));   // (opaque: kept in a register, so that w4_pairs is one logic operation per pair)
 
     for (int pass = 0; pass < passes; ++pass) {
         // this warp's blocks of the pass: the pass's blocks split evenly over the WN warps
@@ -258,22 +261,6 @@ __global__ void __launch_bounds__(W4Shape<CB, WN, NB>::kThreads, 1) proj_w4_kern
                                                                         nb * 8 * (S::kChunk * 2) + kb * 256 + (w >> 1) * 128);
                         x[nb][w][0] = v.x; x[nb][w][1] = v.y; x[nb][w][2] = v.z; x[nb][w][3] = v.w;
                     }
-                // sums of the rows' inputs over each group, by products with ones
-                float xsum[NB][kGroups][2];
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int gr = 0; gr < kGroups; ++gr) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-                        for (int w = gr * GW; w < (gr + 1) * GW; ++w) {
-                            mma_bf16_16816(d, ones, x[nb][w][0], x[nb][w][1]);
-                            mma_bf16_16816(d, ones, x[nb][w][2], x[nb][w][3]);
-                        }
-                        xsum[nb][gr][0] = d[0];
-                        xsum[nb][gr][1] = d[1];
-                    }
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
                     if (cb >= cbs) break;
@@ -292,21 +279,16 @@ __global__ void __launch_bounds__(W4Shape<CB, WN, NB>::kThreads, 1) proj_w4_kern
                     };
 #pragma unroll
                     for (int gr = 0; gr < kGroups; ++gr) {
-                        const float z0 = w4_minus_zero(zraw[0], gr), z1 = w4_minus_zero(zraw[1], gr);
+                        const uint32_t z0 = w4_zero_pair(zraw[0], gr), z1 = w4_zero_pair(zraw[1], gr);
                         float d[NB][4];
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            d[nb][0] = z0 * xsum[nb][gr][0];
-                            d[nb][1] = z0 * xsum[nb][gr][1];
-                            d[nb][2] = z1 * xsum[nb][gr][0];
-                            d[nb][3] = z1 * xsum[nb][gr][1];
-                        }
+                        for (int nb = 0; nb < NB; ++nb) d[nb][0] = d[nb][1] = d[nb][2] = d[nb][3] = 0.0f;
 #pragma unroll
                         for (int wi = 0; wi < GW; ++wi) {
                             const int w = gr * GW + wi;
                             uint32_t pl[4], ph[4];
-                            w4_pairs(*reinterpret_cast<const uint32_t*>(st + woff[kb * 4 + w] + cb * 16 * S::kRow), sixteens, pl);
-                            w4_pairs(*reinterpret_cast<const uint32_t*>(st + woff[kb * 4 + w] + (cb * 16 + 8) * S::kRow), sixteens, ph);
+                            w4_pairs(*reinterpret_cast<const uint32_t*>(st + woff[kb * 4 + w] + cb * 16 * S::kRow), base, z0, pl);
+                            w4_pairs(*reinterpret_cast<const uint32_t*>(st + woff[kb * 4 + w] + (cb * 16 + 8) * S::kRow), base, z1, ph);
                             const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]}, a1[4] = {pl[2], ph[2], pl[3], ph[3]};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) mma_bf16_16816(d[nb], a0, x[nb][w][0], x[nb][w][1]);
