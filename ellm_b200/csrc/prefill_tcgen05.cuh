@@ -1319,6 +1319,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 if constexpr (kExt != 0 && sizeof(OutT) == 2) {
                     unsigned redo = __ballot_sync(0xffffffffu, bad && valid);
+                    __syncwarp();   // each lane's stores of its own row, before other lanes store the same row
                     while (redo) {   // rare: one row at a time, the whole warp on it
                         const int src = __ffs(redo) - 1;
                         redo &= redo - 1;
