@@ -987,6 +987,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         int steps_done = 0;     // key steps of this row tile over all items so far
         bool ok = true;
         Item it;
+        int redo_item = -1;        // kExt: the last item with rows of this warp to be computed again, and which
+        unsigned redo_rows = 0;
         int n_traced = 0;
         for (long long k = 0; ok; ++k) {
             int idx = n_items;
@@ -1318,19 +1320,17 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (valid && p.lse) p.lse[row_index] = (m_used + log2f(l)) * kLn2;
                 }
                 if constexpr (kExt != 0 && sizeof(OutT) == 2) {
-                    unsigned redo = __ballot_sync(0xffffffffu, bad && valid);
+                    // These rows are computed again once the list is done: doing it here would keep the other roles in
+                    // their bounded waits.  The warp's items with such rows form a chain through the rows' own outputs.
+                    const unsigned redo = __ballot_sync(0xffffffffu, bad && valid);
                     __syncwarp();   // each lane's stores of its own row, before other lanes store the same row
-                    while (redo) {   // rare: one row at a time, the whole warp on it
-                        const int src = __ffs(redo) - 1;
-                        redo &= redo - 1;
-                        const int r_pos = __shfl_sync(0xffffffffu, pos, src), r_head = it.kvh * p.group + __shfl_sync(0xffffffffu, g, src);
-                        const long long r_index = __shfl_sync(0xffffffffu, row_index, src);
-                        const ScoreMods& m = p.ext.mods;
-                        exact_row(m, p.ext.q + r_index * kHeadDim, p.ext.k + it.b * p.ext.s0 + it.kvh * p.ext.s1,
-                                  p.ext.v + it.b * p.ext.s0 + it.kvh * p.ext.s1, p.ext.s2, m.pk + it.kvh * m.ps1, m.pv + it.kvh * m.ps1,
-                                  it.base + r_pos, __shfl_sync(0xffffffffu, row_lo, src), __shfl_sync(0xffffffffu, row_hi, src),
-                                  m.slopes ? m.slopes[r_head] * kLog2e : 0.0f,
-                                  reinterpret_cast<__nv_bfloat16*>(p.out) + r_index * kHeadDim, p.lse ? p.lse + r_index : nullptr, lane);
+                    if (redo) {
+                        const long long r_index = __shfl_sync(0xffffffffu, row_index, __ffs(redo) - 1);
+                        if (lane == 0)
+                            *reinterpret_cast<int2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + r_index * kHeadDim) =
+                                make_int2(redo_item, static_cast<int>(redo_rows));
+                        redo_item = idx;
+                        redo_rows = redo;
                     }
                 }
                 // the next item's first P.V overwrites O_t: its P is only handed over by these same
@@ -1351,6 +1351,32 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             steps_done += my_steps;
             if ((warp & 3) == 0 && lane == 0) TC_TRACE(tr + 3);
+        }
+        if constexpr (kExt != 0 && !kSplit && sizeof(OutT) == 2) {
+            // Rare: the rows that came out not finite, key by key (see exact_row), one row at a time, the whole warp on
+            // it.  Nothing waits for this warp any more but the block's last barrier.
+            while (ok && redo_item >= 0) {
+                tc_item(p, redo_item, it);
+                const int rho0 = (it.pair * kTcTiles + t) * p.ext.tile_pos * p.group + (warp & 3) * 32;   // of lane 0
+                auto row_at = [&](int rho) { return (static_cast<long long>(rho / p.group) * p.max_batch + it.b) * p.q_heads + it.kvh * p.group + rho % p.group; };
+                __nv_bfloat16* const out = reinterpret_cast<__nv_bfloat16*>(p.out);
+                int2 link = make_int2(-1, 0);
+                if (lane == 0) link = *reinterpret_cast<const int2*>(out + row_at(rho0 + __ffs(redo_rows) - 1) * kHeadDim);   // (written by this lane)
+                link.x = __shfl_sync(0xffffffffu, link.x, 0);
+                link.y = __shfl_sync(0xffffffffu, link.y, 0);
+                const ScoreMods& m = p.ext.mods;
+                for (unsigned rows = redo_rows; rows; rows &= rows - 1) {
+                    const int rho = rho0 + __ffs(rows) - 1, head = it.kvh * p.group + rho % p.group;
+                    const long long r_index = row_at(rho), r_pos = it.base + rho / p.group;
+                    long long lo, hi;
+                    row_interval(m, it.b, r_pos, it.key_end, lo, hi);
+                    exact_row(m, p.ext.q + r_index * kHeadDim, p.ext.k + it.b * p.ext.s0 + it.kvh * p.ext.s1,
+                              p.ext.v + it.b * p.ext.s0 + it.kvh * p.ext.s1, p.ext.s2, m.pk + it.kvh * m.ps1, m.pv + it.kvh * m.ps1, r_pos, lo, hi,
+                              m.slopes ? m.slopes[head] * kLog2e : 0.0f, out + r_index * kHeadDim, p.lse ? p.lse + r_index : nullptr, lane);
+                }
+                redo_item = link.x;
+                redo_rows = static_cast<unsigned>(link.y);
+            }
         }
     } else if (warp == kTcTiles * 4) {
         // =============================== TMA producer ===============================
