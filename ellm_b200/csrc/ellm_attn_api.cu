@@ -1214,7 +1214,7 @@ int ellm_step_graph_destroy(ellm_step_graph* g) {
     return ELLM_OK;
 }
 
-// The captured host-buffer step holds the scores and the prefix it was captured with: built anew after a change.
+// The captured host-buffer step holds the scores, the prefix and the options it was captured with: built anew after a change.
 static void drop_host_step(ellm_attn* h) {
     DeviceGuard guard(h->d.device);
     if (h->graph_exec) cudaGraphExecDestroy(h->graph_exec);
@@ -1318,6 +1318,7 @@ int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size
 int ellm_attn_set_option(ellm_attn* h, const char* name, long long value) {
     if (!h || !name) return fail(ELLM_ERR_INVALID_ARG, "handle and name must be non-NULL");
     std::lock_guard<std::mutex> lock(h->mu);
+    drop_host_step(h);   // it holds the limits, the grid and the choice of kernels that it was captured with
     if (std::strcmp(name, "tc_wait_timeout_ns") == 0) {
         if (value <= 0) return fail(ELLM_ERR_INVALID_ARG, "tc_wait_timeout_ns must be > 0");
         h->tc.wait_timeout_ns = static_cast<unsigned long long>(value);
