@@ -632,6 +632,19 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
     const size_t lda = d.a_row_stride ? d.a_row_stride : d.k_max;
     const long long ldc = static_cast<long long>(d.output_row_stride ? d.output_row_stride : d.n_max);
     const long long ldr = static_cast<long long>(d.residual_row_stride ? d.residual_row_stride : d.n_max);
+    cudaEvent_t e0 = nullptr, e1 = nullptr;   // around the run's launches when profiling is on
+    if (h->profiling) {
+        ELLM_CUDA(cudaEventCreate(&e0));
+        ELLM_CUDA(cudaEventCreate(&e1));
+        ELLM_CUDA(cudaEventRecord(e0, h->stream));
+    }
+    auto launched = [&]() -> int {
+        if (e1) {
+            ELLM_CUDA(cudaEventRecord(e1, h->stream));
+            h->pending.emplace_back(e0, e1);
+        }
+        return proj_finish(h);
+    };
     if (rows <= static_cast<size_t>(ellm::kW4MaxRows) && !w4_use_tc(h, rows)) {
         ellm::W4Params p{};
         p.a = static_cast<const __nv_bfloat16*>(d.a);
@@ -652,7 +665,7 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
         const unsigned grid = static_cast<unsigned>(std::min<size_t>((d.n_max + 15) / 16, static_cast<size_t>(h->plan.sm_count)));
         ELLM_CUDA(launch_dependent(c.kernel, grid, static_cast<unsigned>(c.threads), static_cast<size_t>(c.smem), h->stream, p));
         ++h->skinny_launches;
-        return proj_finish(h);
+        return launched();
     }
     const size_t tiles_m = rows <= 32 ? 1 : (rows + 255) / 256;
     const int mt = rows <= 16 ? 16 : rows <= 32 ? 32 : static_cast<int>(((rows + tiles_m - 1) / tiles_m + 15) / 16 * 16);
@@ -700,7 +713,7 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
         ELLM_CUDA(cudaLaunchKernelEx(&cfg, ellm::w4_reduce_kernel, p, static_cast<int>(ctas)));
         ++h->launches;
     }
-    return proj_finish(h);
+    return launched();
 }
 
 static ProjHandle* proj_cast(void* handle, int which) {

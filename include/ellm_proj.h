@@ -159,7 +159,8 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
                            size_t cpu_num, size_t thread_id);
 
 /* Launches and device time of a handle's kernel since profiling was switched on (events around
- * every launch; for measurement only).  `which`: 0 = ellm_matmul3, 1 = ellm_matmul_add,
+ * every launch of the tensor-memory kernel, or around all launches of an ellm_matmul_add_w4 run, which
+ * count as one timed launch; for measurement only).  `which`: 0 = ellm_matmul3, 1 = ellm_matmul_add,
  * 2 = ellm_matmul_add_w4. */
 int ellm_matmul_set_profiling(void* handle, int which, int on);
 int ellm_matmul_kernel_stats(void* handle, int which, uint64_t* launches, uint64_t* timed_launches, double* ms);
