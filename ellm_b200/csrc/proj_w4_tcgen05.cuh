@@ -251,6 +251,7 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                 for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(wp + ((i ^ ((lane >> 1) & 3)) << 4));
                 slot = slot + 1 == kRing ? 0 : slot + 1;
                 const int b = static_cast<int>(n_done & 3);
+                if ((n_done & ~1u) == 4u) asm volatile("griddepcontrol.wait;" ::: "memory");   // from here on the wait is for products (see below)
                 if (lane == 0)
                     ok = mbar_wait(bar_un_empty(b), ((n_done >> 2) & 1u) ^ 1u, abort_word, p.status, kWtWaitUnpackedEmpty, p.wait_timeout_ns);
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;   // (also: every lane has read its packed words)
@@ -314,6 +315,9 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
         // The whole warp walks the list, so that descriptors and addresses stay in uniform registers, and one elected
         // lane issues.  A block's barriers are waited for side by side, a lane each (one after the other each costs about
         // 100 clocks even when it is ready).  With one lane doing everything a block took 1100 clocks, whatever the rows.
+        // The products need the rows, which are copied in once the previous kernel has finished: that is waited for ahead
+        // of the first wait that has a limit, here and in the other roles, so that its time does not count against it.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         bool ok = true;
         unsigned n_done = 0, n_acc = 0;   // blocks; accumulators handed over
         int s = 0;
@@ -365,14 +369,11 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
         const int r = (warp & 3) * 32 + lane;   // tensor-memory lane = weight row of the tile
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         unsigned n_done = 0, n_acc = 0;
-        bool ok = true, waited = false;
+        bool ok = true;
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // also: outputs, parts and the residual belong to earlier kernels until here
         for (long long u = u0; ok && w4_segment(p, u, u0, u1, sg); u += sg.blocks) {
             const int n = sg.tile_n * kWtTileN + r, m0 = sg.tile_m * mt;
             const bool exists = n < p.n_cols;
-            auto before_store = [&]() {   // outputs, parts and the residual belong to earlier kernels until here
-                if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-                waited = true;
-            };
             // rows m .. m + 15 of this weight row (the residual's values requested together)
             const bool all_live = p.batch == p.max_batch;
             auto store16 = [&](int m, float* v) {
@@ -436,7 +437,6 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                     if (lane == 0) mbar_arrive(bar_acc_empty(b));
                 }
                 if (!ok) break;
-                before_store();
 #pragma unroll
                 for (int m = 0; m < kMt; m += 16) store16(m, acc + m);
             } else {
@@ -444,7 +444,6 @@ proj_w4_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const uint8_t*
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                 if (!ok) break;
                 tc_fence_after();
-                before_store();
                 for (int m = 0; m < mt; m += 16) {
                     float v[16];
                     tmem_ld16(tmem + lane_base + 256 + m, v);
