@@ -111,9 +111,11 @@ __device__ __forceinline__ int dec_tiles_of(long long begin, long long len) {
 // kDecPrefix: a shared prefix, as segments (KV head, block of 16 of the step's query rows) behind the sequences' own
 // in the same tile list - the prefix is read once per 16 query rows, mostly from L2, by the one launch there
 // is anyway.  (Steps with more work take the tensor-memory kernel for the prefix, see launch_decode.)
-// kDecBehind: the launch right before is the tensor-memory kernel of the shared prefix, which lets this grid start once
-// everything before it has finished: nothing to wait for at the start, and the end waits for that kernel, so that
-// the merge behind this grid finds both.
+// kDecBehind: the launch right before is the tensor-memory kernel of the shared prefix.  Each of its blocks waits for
+// everything before it, fences and only then lets this grid start, which fences before its first read: positions,
+// queries and rows of kernels further back are seen although this grid does not wait for its predecessor at the start
+// (it reads nothing of that one's; waiting there costs 4 to 10 us a step, both fences less than 1).  The end waits for that
+// kernel, so that the merge behind this grid finds both.
 enum { kDecPlain = 0, kDecMods = 1, kDecPrefix = 2, kDecBehind = 3 };
 
 // kMods: the keys start at row_begin[b][position]; begs[b] receives that (where begs is given).
@@ -239,6 +241,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) decode_splitkv_kernel(const De
     // With early streaming the wait comes later, after the first stages have been requested.
     bool waited = p.early == 0 || kKind == kDecBehind;
     if constexpr (kKind == kDecBehind) {
+        __threadfence();   // the other half of the fence ahead of that kernel's trigger: nothing older is read from this SM's L1
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     } else if (waited) {
         asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -962,8 +962,11 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // was still at work; everything below reads or writes what that kernel may have touched.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // the split-KV kernel behind this one reads nothing that this one writes: from here on it may run, and only
-    // its end waits for this grid's
-    if constexpr (kSplit) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // its end waits for this grid's.  What older kernels wrote is visible here; the fence passes that on.
+    if constexpr (kSplit) {
+        __threadfence();
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     if (threadIdx.x == 0) TC_TRACE(2);
     const int total_rows = p.interval * p.group;
     const int n_items = static_cast<int>(p.n_items);
