@@ -35,7 +35,7 @@
 // in the same one-pass step.  The interval hulls come from a table filled by a small kernel ahead
 // of this one (row_begin), or follow from the positions alone.
 // What bounds it: the softmax warps.  A 128-key step of both row tiles takes about 3700 clocks plain, 5000 capped
-// (five multiply-adds a score for the tanh) and 4300 biased, against 2800 for its products; an item costs about
+// (six multiply-adds a score for the tanh) and 4300 biased, against 2800 for its products; an item costs about
 // 11000 clocks besides its steps (queries, first tile, epilogue), which is what short documents and windows pay.
 // Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.55 ms (862 TFLOP/s); 2 x 8191 tokens of
 // documents of about 900, biased, 32 / 8 heads, 365 us; 8 x 256 rows under a capped 1024-key window, 64 / 8 heads, 140 us;
@@ -116,11 +116,11 @@ struct Tcgen05Plan {
     CUtensorMap ext_q, ext_k, ext_v, ext_pk, ext_pv;
 };
 
-// kExt, capped scores: above kTcCapMax the polynomial's 7e-6 of a score of cap would pass a quarter of P's rounding
-// to bf16 (such chunks go to the warp-level kernel); up to kTcFixedMaxCap in log2 units the softmax takes 0 for the
-// row maximum: exp2 of +-88 and sums of 2^20 such are far from the ends of fp32's range.
-// (cap_in's 9th power is folded into a coefficient: it has to stay in fp32's range)
-constexpr float kTcCapMax = 128.0f, kTcCapInMin = 1.0f / 4096.0f, kTcCapInMax = 4096.0f;
+// kExt, capped scores: the form used past the polynomial's range is off by 1e-7 of cap whatever the score, which above
+// kTcCapMax would pass 1e-5 of an exponent (such chunks go to the warp-level kernel); up to kTcFixedMaxCap in log2 units the
+// softmax takes 0 for the row maximum: exp2 of +-88 and sums of 2^20 such are far from the ends of fp32's range.
+// (cap_in's 11th power is folded into a coefficient: it has to stay in fp32's range)
+constexpr float kTcCapMax = 128.0f, kTcCapInMin = 1.0f / 4096.0f, kTcCapInMax = 2048.0f;
 constexpr float kTcFixedMaxCap = 88.0f;
 // kExt bits
 enum { kExtOn = 1, kExtCap = 2, kExtBias = 4, kExtSplit = 8 };
@@ -133,7 +133,7 @@ struct TcExt {
     int prefix_tiles = 0;           // 128-key tiles of the shared prefix
     int splits = 1;                 // kExtSplit: runs of prefix tiles, each with its own partial result
     long long part_rows = 0;        // kExtSplit: rows of one partial
-    float cap_coef[5] = {};         // the tanh polynomial in the product itself: coefficient of t^(2i+1), times cap_log2
+    float cap_coef[6] = {};         // the tanh polynomial in the product itself: coefficient of t^(2i+1), times cap_log2
     // q and the cache, for the rows recomputed key by key
     const __nv_bfloat16* q = nullptr;
     const __nv_bfloat16* k = nullptr;
@@ -693,7 +693,7 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
 //   kCap: the tanh polynomial with cap_in folded into its coefficients;  kScored: s holds scores already.
 //   m0, m1: visible columns;  base, slope: the distance bias of column i is base + slope * i (kExtBias, `ahead`).
 template <int kExt, bool kScored, bool kMask>
-__device__ __forceinline__ float tc_exp64(const float (&s)[64], const TcRow& r, const float (&coef)[5], float base, unsigned m0, unsigned m1,
+__device__ __forceinline__ float tc_exp64(const float (&s)[64], const TcRow& r, const float (&coef)[6], float base, unsigned m0, unsigned m1,
                                           uint32_t (&pk)[32]) {
     const uint64_t base2 = pack2(base, base), scale2 = pack2(r.scale_log2, r.scale_log2);
     uint64_t sum_a = pack2(0.0f, 0.0f), sum_b = sum_a;
@@ -707,7 +707,8 @@ __device__ __forceinline__ float tc_exp64(const float (&s)[64], const TcRow& r, 
             x2 = add2(s2, base2);
         } else if constexpr ((kExt & kExtCap) != 0) {
             const uint64_t v = mul2(s2, s2);
-            uint64_t q = fma2(pack2(coef[4], coef[4]), v, pack2(coef[3], coef[3]));
+            uint64_t q = fma2(pack2(coef[5], coef[5]), v, pack2(coef[4], coef[4]));
+            q = fma2(q, v, pack2(coef[3], coef[3]));
             q = fma2(q, v, pack2(coef[2], coef[2]));
             q = fma2(q, v, pack2(coef[1], coef[1]));
             q = fma2(q, v, pack2(coef[0], coef[0]));
@@ -731,7 +732,7 @@ __device__ __forceinline__ float tc_exp64(const float (&s)[64], const TcRow& r, 
     return sa + sb;
 }
 template <int kExt>
-__device__ __forceinline__ float tc_row64(float (&s)[64], const TcRow& r, const float (&coef)[5], float c0, float off, bool edge, int lo, int rel,
+__device__ __forceinline__ float tc_row64(float (&s)[64], const TcRow& r, const float (&coef)[6], float c0, float off, bool edge, int lo, int rel,
                                           uint32_t (&pk)[32]) {
     unsigned m0 = ~0u, m1 = ~0u;
     if (edge) {
@@ -844,7 +845,7 @@ __device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRo
 // One key tile of a kExt row tile: P_t in tensor memory on return.  fixed_max: the scores are bounded (capped, no
 // bias), m_used is a constant for the whole row and nothing can leap.
 template <int kExt>
-__device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRow& r, const float (&coef)[5], int lo, int rel, bool edge,
+__device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRow& r, const float (&coef)[6], int lo, int rel, bool edge,
                                             bool first, bool fixed_max, bool valid, float& m_used, float& l) {
     bool slow = false;
     if (!fixed_max && __any_sync(0xffffffffu, m_used == -INFINITY && valid)) {
@@ -1012,7 +1013,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // kExt: the row's interval of own keys, its constants
             int row_lo = 0, row_hi = 0;
             TcRow xr{};
-            float coef[5] = {};
+            float coef[6] = {};
             bool fixed_max = false;
             if constexpr (kExt != 0) {
                 if ((kExt & kExtSplit) == 0 && valid) {
@@ -1027,7 +1028,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if ((kExt & kExtBias) && valid) xr.slope = p.ext.mods.slopes[it.kvh * p.group + g] * kLog2e;
                 if constexpr ((kExt & kExtCap) != 0)
 #pragma unroll
-                    for (int i = 0; i < 5; ++i) coef[i] = p.ext.cap_coef[i];
+                    for (int i = 0; i < 6; ++i) coef[i] = p.ext.cap_coef[i];
                 // capped scores lie in +-cap: with 2^(cap log2 e) far inside fp32's (and bf16's) range the softmax needs no maximum
                 fixed_max = (kExt & kExtCap) && !(kExt & kExtBias) && p.ext.mods.cap_log2 <= kTcFixedMaxCap;
             }
@@ -2212,8 +2213,8 @@ inline int launch_prefill_tcgen05_ext(Tcgen05Plan& plan, const ellm_attn_desc& d
     p.ext.tile_pos = tile_pos;
     p.ext.tiles = static_cast<int>((interval + tile_pos - 1) / tile_pos);
     p.ext.prefix_tiles = static_cast<int>((mods.plen + kTcKeys - 1) / kTcKeys);
-    const float c[5] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4};
-    for (int i = 0; i < 5; ++i) p.ext.cap_coef[i] = static_cast<float>(c[i] * std::pow(static_cast<double>(mods.cap_in), 2 * i + 1) * mods.cap_log2);
+    const float c[6] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4, kTanhC5};
+    for (int i = 0; i < 6; ++i) p.ext.cap_coef[i] = static_cast<float>(c[i] * std::pow(static_cast<double>(mods.cap_in), 2 * i + 1) * mods.cap_log2);
     p.ext.q = static_cast<const __nv_bfloat16*>(d.q);
     p.ext.k = static_cast<const __nv_bfloat16*>(d.k_cache);
     p.ext.v = static_cast<const __nv_bfloat16*>(d.v_cache);

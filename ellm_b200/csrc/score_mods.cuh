@@ -13,11 +13,11 @@
 // The tanh.  cap * tanh shifts an exponent, so what counts is the error of the product: relative to the
 // score where the cap hardly bends it, absolute where it saturates.  Two forms, both odd polynomials
 // (least-squares fits of P(u) / tanh(u) reweighted to equal ripple) near zero:
-//   * any u: 4 terms for |u| < 1/4 (relative error 2.5e-9), 1 - 2 / (1 + e^(2u)) beyond (1e-7 absolute);
+//   * any u: 4 terms for |u| < 1/4 (2.5e-9 off before fp32's own roundings), 1 - 2 / (1 + e^(2u)) beyond (1e-7 absolute);
 //     two special-function operations per score;
-//   * 5 terms for |u| <= 1 (relative error 6.9e-6: 4e-4 of an exponent at a score of 40 under cap 50, where
-//     P is rounded by up to 4e-3), on packed pairs and without the special-function unit, which is what the
-//     chunk kernel is short of.  That kernel takes it whenever 64 scores of each row of a warp are in range.
+//   * 6 terms for |u| <= 1 (relative error 6.1e-7: 6e-5 of an exponent at cap 128; five terms have 6.9e-6), on packed
+//     pairs and without the special-function unit, which is what the chunk kernel is short of.  That kernel takes it
+//     whenever 64 scores of each row of a warp are in range.
 #pragma once
 #include "common.cuh"
 
@@ -52,10 +52,10 @@ __device__ __forceinline__ float fast_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// coefficients of u, u^3, ..., u^9 of the polynomial for |u| <= kTanhPolyMax
+// coefficients of u, u^3, ..., u^11 of the polynomial for |u| <= kTanhPolyMax
 constexpr float kTanhPolyMax = 1.0f;
-constexpr float kTanhC0 = 0.9999930859f, kTanhC1 = -0.3329806626f, kTanhC2 = 0.1303680986f, kTanhC3 = -0.0448175333f,
-                kTanhC4 = 0.0090364163f;
+constexpr float kTanhC0 = 0.9999994040f, kTanhC1 = -0.3332904279f, kTanhC2 = 0.1328143328f, kTanhC3 = -0.0516056642f,
+                kTanhC4 = 0.0167431068f, kTanhC5 = -0.0030670569f;
 // tanh of any argument (saturates through e^(2u) = 0 and infinity; NaN stays NaN)
 __device__ __forceinline__ float tanh_any(float u) {
     const float v = u * u;

@@ -267,7 +267,7 @@ int ellm_step_graph_destroy(ellm_step_graph* graph);
  *                rows (pos + 1: empty).  Values below 0 count as 0.
  *   prefix_lens  the first prefix_lens[b] positions are seen by all rows of sequence b, earlier rows
  *                included; they have to lie in one chunk (a row cannot see keys not yet written).
- * Two things are right but slow: chunks with softcap > 128 (or scale / softcap outside [1/4096, 4096]) run
+ * Two things are right but slow: chunks with softcap > 128 (or scale / softcap outside [1/4096, 2048]) run
  * on the warp-level kernel, and rows whose 128-key tiles hold NaN or infinity are computed once more, key by key.
  * All arrays are device memory, read by every run; they have to stay valid and may be rewritten between
  * runs.  The distance is that of positions in the handle's cache.  The struct is copied; s NULL, or one
