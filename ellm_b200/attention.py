@@ -141,7 +141,8 @@ class Attention:
     def set_shared_prefix(self, k, v, prefix_len=None, strides=None):
         """A prefix shared by all sequences of the batch (ellm_attn_set_shared_prefix): k and v
         [kv_heads, rows, head_size] bf16, of which the first prefix_len rows count (default: all).  The handle's
-        cache and positions then count what follows the prefix.  With raw pointers, strides = (kv head, position)
+        cache and positions then count what follows the prefix, so a projection that rotates takes the table from row
+        prefix_len on (rope_ptr=rope[prefix_len:]).  With raw pointers, strides = (kv head, position)
         in elements.  k = None removes it."""
         if k is None:
             L.check(self._lib.ellm_attn_set_shared_prefix(self._h, None, None, 0, 0, 0))

@@ -289,8 +289,12 @@ int ellm_attn_set_scores(ellm_attn* h, const ellm_attn_scores* s);
  * row * position_stride + c, bf16 - for instance one sequence's slot of another cache.  Afterwards the
  * handle's cache and positions count what FOLLOWS the prefix: the row at position p of sequence b
  * attends all prefix rows and cache rows 0..=p of its sequence (with p = -1 in run_ragged: the prefix
- * alone).  The prefix is read once for the whole batch, not once per sequence, in decode steps of any
- * batch.  k NULL or prefix_len 0 removes it.  Not together with ellm_attn_set_scores nor
+ * alone).  A projection that rotates takes the same positions: give ellm_matmul3 and
+ * ellm_qk_norm_rope_append the rotation table from row prefix_len on (rope + prefix_len * 128, rope_rows -
+ * prefix_len), or queries and new keys are rotated as if the prefix were not there; the prefix's own rows
+ * are rotated at positions 0 .. prefix_len - 1.  A decode step reads the prefix once per 16 or per 256 query
+ * rows of a KV head (of all sequences together), not once per sequence; a chunk reads it with every 256 rows
+ * of a sequence and KV head.  k NULL or prefix_len 0 removes it.  Not together with ellm_attn_set_scores nor
  * ellm_attn_run_window (ELLM_ERR_UNSUPPORTED).  May allocate workspace; calls on a handle must not
  * overlap, and graphs captured before the call keep what they captured.  No counterpart in the
  * reference (one private K/V buffer per sequence slot, src/memory/cache.rs:69-75). */
