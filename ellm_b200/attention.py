@@ -33,6 +33,16 @@ def _check_tensor(name, t, dtype, shape, device):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on CUDA device {device}")
 
 
+def _reads(desc, *tensors):
+    """Tells torch that an enqueue-only operator reads these tensors on its own stream, so that their memory is not handed
+    out again while queued steps still read it after the operator let go of them (raw pointers are their owner's)."""
+    for t in tensors if desc.async_ else ():
+        if hasattr(t, "record_stream"):
+            import torch
+            device = torch.device("cuda", desc.device)
+            t.record_stream(torch.cuda.ExternalStream(desc.stream, device) if desc.stream else torch.cuda.default_stream(device))
+
+
 class Attention:
     def __init__(self):
         raise TypeError("use Attention.new(...)")
@@ -120,8 +130,9 @@ class Attention:
         softcap: s -> softcap * tanh(s / softcap) (0 = none).  slopes: float32 [q_heads], s -> s - slopes[h] *
         |pos - key|.  row_begin: int32 [max_batch, >= max_seq], the first key the row at each position sees
         (document start, window start, pos + 1 for a row that sees nothing).  prefix_lens: int32 [max_batch],
-        positions every row of the sequence sees.  Tensors are device buffers read by every run; without any
-        argument the operator goes back to plain attention."""
+        positions every row of the sequence sees.  Tensors are device buffers read by every run (and by every replay of
+        a graph captured with them: they have to outlive it); without any argument the operator goes back to plain
+        attention."""
         d = self.desc
         _check_tensor("slopes", slopes, "float32", (d.q_heads,), d.device)
         _check_tensor("prefix_lens", prefix_lens, "int32", (d.max_batch,), d.device)
@@ -137,13 +148,14 @@ class Attention:
         s = L.AttnScores(float(softcap), _ptr(slopes), _ptr(row_begin), stride, _ptr(prefix_lens))
         L.check(self._lib.ellm_attn_set_scores(self._h, C.byref(s)))
         self._keep_scores = (slopes, row_begin, prefix_lens)
+        _reads(d, *self._keep_scores)
 
     def set_shared_prefix(self, k, v, prefix_len=None, strides=None):
         """A prefix shared by all sequences of the batch (ellm_attn_set_shared_prefix): k and v
         [kv_heads, rows, head_size] bf16, of which the first prefix_len rows count (default: all).  The handle's
         cache and positions then count what follows the prefix, so a projection that rotates takes the table from row
         prefix_len on (rope_ptr=rope[prefix_len:]).  With raw pointers, strides = (kv head, position)
-        in elements.  k = None removes it."""
+        in elements.  Captured graphs read the tensors too: they have to outlive them.  k = None removes it."""
         if k is None:
             L.check(self._lib.ellm_attn_set_shared_prefix(self._h, None, None, 0, 0, 0))
             self._keep_prefix = None
@@ -169,6 +181,7 @@ class Attention:
         L.check(self._lib.ellm_attn_set_shared_prefix(self._h, _ptr(k), _ptr(v), int(strides[0]), int(strides[1]),
                                                       int(prefix_len)))
         self._keep_prefix = (k, v)
+        _reads(self.desc, k, v)
 
     def set_option(self, name, value):
         L.check(self._lib.ellm_attn_set_option(self._h, name.encode(), int(value)))
