@@ -160,6 +160,8 @@ class Attention:
             L.check(self._lib.ellm_attn_set_shared_prefix(self._h, None, None, 0, 0, 0))
             self._keep_prefix = None
             return
+        if hasattr(k, "data_ptr") != hasattr(v, "data_ptr"):
+            raise ValueError("k and v must both be tensors or both raw pointers")
         if hasattr(k, "data_ptr"):
             for name, t in (("k", k), ("v", v)):
                 if str(t.dtype) != "torch.bfloat16" or not _on_device(t, self.desc.device) or t.dim() != 3 or t.stride(2) != 1 \
@@ -172,10 +174,12 @@ class Attention:
                 prefix_len = k.shape[1]
             if not 0 <= prefix_len <= k.shape[1]:
                 raise ValueError(f"prefix_len {prefix_len} outside [0, {k.shape[1]}]")
-            if strides is None:
-                # (strides over one head or one row say nothing)
-                ps = k.stride(1) if k.shape[1] > 1 else k.shape[2]
-                strides = (k.stride(0) if k.shape[0] > 1 else k.shape[1] * ps, ps)
+            # (strides over one head or one row say nothing)
+            ps = k.stride(1) if k.shape[1] > 1 else k.shape[2]
+            own = (k.stride(0) if k.shape[0] > 1 else k.shape[1] * ps, ps)
+            if strides is not None and tuple(strides) != own:
+                raise ValueError(f"strides go with raw pointers: those of the tensors are {own}")
+            strides = own
         if prefix_len is None or strides is None:
             raise ValueError("raw pointers need prefix_len and strides")
         L.check(self._lib.ellm_attn_set_shared_prefix(self._h, _ptr(k), _ptr(v), int(strides[0]), int(strides[1]),
