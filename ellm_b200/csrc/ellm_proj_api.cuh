@@ -628,7 +628,7 @@ int ellm_matmul_add_w4_run(ellm_matmul_add_w4* h, size_t position_index, size_t 
     std::lock_guard<std::mutex> lock(h->mu);
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(ELLM_ERR_CUDA, "cannot select device %d", h->device);
-    const size_t rows = position_interval * d.max_batch;
+    const size_t rows = (position_interval - 1) * d.max_batch + batch_size;   // up to the last live one
     const size_t lda = d.a_row_stride ? d.a_row_stride : d.k_max;
     const long long ldc = static_cast<long long>(d.output_row_stride ? d.output_row_stride : d.n_max);
     const long long ldr = static_cast<long long>(d.residual_row_stride ? d.residual_row_stride : d.n_max);

@@ -137,7 +137,9 @@ class MatMulAddW4(_Projection):
             a_row_stride=0, residual_row_stride=0, output_row_stride=0, device=0, stream=None, async_=False):
         """output = ptr3 (residual, may be None) + ptr1 [m, k] . W^T, W[n, k] = (q[n, k] - z) * scale with one
         scale (and zero point) per `group` inputs: w4_ptr uint8 [n, k / 2] as pack_int4 lays it out, scales_ptr
-        bf16 [n, k / group], zeros uint8 [n, k / group] or None (8 everywhere)."""
+        bf16 [n, k / group], zeros uint8 [n, k / group] with numbers 0..127 or None (8 everywhere).  Runs whose last
+        live row is beyond the 32nd multiply by W rounded to bf16, shorter ones by q - z with the scale on the fp32
+        sums.  A handle keeps 2 x SMs x min(256, m_max) x 512 bytes of workspace."""
         self = object.__new__(cls)
         self._h = None
         lib = L.load()

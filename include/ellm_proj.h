@@ -122,8 +122,9 @@ int ellm_matmul_add_run(ellm_matmul_add* h, size_t position_index, size_t positi
 /* ---- MatMulAddW4: output = residual + A . W^T with 4-bit weights --------------------------------
  * MatMulAdd for a checkpoint whose weights are 4-bit numbers with one scale per group of inputs:
  *     W[n][k] = (q[n][k] - z[n][k / group]) * scale[n][k / group],   q in 0..15.
- * The sum is formed in fp32 and rounded to bf16 once; runs of at most 32 rows multiply by q - z and
- * apply the scale to the fp32 sums, larger ones multiply by W rounded to bf16.  Weights, scales and
+ * The sum is formed in fp32 and rounded to bf16 once; runs of at most 32 rows multiply by q - z, exactly,
+ * and apply the scale to the fp32 sums, larger ones multiply by W rounded to bf16.  Rows are counted up to the
+ * last live one, (position_interval - 1) * max_batch + batch_size, idle ones between live ones included.  Weights, scales and
  * zero points are read by every run, in place, and (like the weights of the other projections in a decode
  * step) ahead of the wait for the stream's previous kernel: after a kernel that rewrites them, wait for the
  * stream before the next run.  A handle keeps 2 x SMs x min(256, m_max) x 128 fp32 of workspace, so runs of
