@@ -545,10 +545,11 @@ W4Choice w4_choice(size_t n, size_t group, int sm_count) {
     return w4_choice_of<4, 4, NB>(group);
 }
 
-// Up to 16 rows both forms give the same sums (to fp32).  The warp-level one is a single launch whose warps share a
-// column's K, the tensor-memory one unpacks with fewer instructions per weight but has to add up cut tiles in a
-// second launch.  Measured (us, warp-level / tensor-memory): 8192 x 8192, 8 rows 20.1 / 22.9, 13 rows 27.3 / 23.0;
-// 28672 x 8192, 8 rows 57.8 / 55.8, 13 rows 69.5 / 56.0; 5120 x 2048, 13 rows 8.5 / 11.9.
+// Up to 16 rows both forms multiply q - z and give the same sums (to fp32).  The warp-level one is a single launch whose
+// warps share a column's K, the tensor-memory one unpacks with fewer instructions per weight but has to add up cut tiles
+// in a second launch.  Measured (us, warp-level / tensor-memory), groups of 128: 8192 x 8192, 8 rows 19.4 / 23.0, 13 rows
+// 24.8 / 23.0; 28672 x 8192, 8 rows 60.8 / 56.5, 13 rows 70.6 / 56.4; 5120 x 2048, 13 rows 7.1 / 11.4; 4096 x 4096, 16 rows
+// 8.7 / 13.7.  Groups of 64 lie the same way; with groups of 32 the two are closer: 27.1 / 30.9 and 83.8 / 85.0 for 13 rows.
 bool w4_use_tc(const ProjHandle* h, size_t rows) {
     if (h->plan.pairing >= 0) return h->plan.pairing != 0;
     return static_cast<long long>(h->dw.n_max) * static_cast<long long>(h->dw.k_max) * (rows > 8 ? 4 : 1) >= (1ll << 27);
