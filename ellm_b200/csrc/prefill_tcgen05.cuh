@@ -37,7 +37,7 @@
 // What bounds it: the softmax warps.  A 128-key step of both row tiles takes about 3700 clocks plain, 5000 capped
 // (six multiply-adds a score for the tanh) and 4300 biased, against 2800 for its products; an item costs about
 // 11000 clocks besides its steps (queries, first tile, epilogue), which is what short documents and windows pay.
-// Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.6 to 2.75 ms by the box's clocks (800 to 850
+// Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.6 to 2.75 ms by the GPU's clocks (800 to 850
 // TFLOP/s); 2 x 8191 tokens of documents of about 900, biased, 32 / 8 heads, 373 us; 8 x 256 rows under a capped 1024-key
 // window, 64 / 8 heads, 141 us; 16 x 48 rows after 8190 shared keys, 32 / 4 heads, 162 us (640 TFLOP/s).
 // An item owns all keys of its rows: a chunk of fewer items than SMs leaves the others idle (1 x 64 rows after 8190 keys is
@@ -415,8 +415,6 @@ struct TcItemExt : TcItem {
     int p0 = 0, split = 0;   // kExtSplit: first prefix tile of the item's run
     int flo[kTcTiles], fhi[kTcTiles];
 };
-__device__ __forceinline__ int tc_prefix_tiles(const TcItem&) { return 0; }
-__device__ __forceinline__ int tc_prefix_tiles(const TcItemExt& it) { return it.np; }
 
 // The items are numbered heaviest first: later row tiles have more keys.  When all heads' K/V fit
 // in L2 together the order is heaviest-first over the whole launch, else head by head so that one
@@ -982,7 +980,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
     // Every role walks the same list of items.  What carries over from one item to the next are the
     // barriers' phases, so each role counts what it has pushed through them so far: ring items,
-    // key steps per row tile, Q loads per row tile, tail clean-ups.
+    // key steps per row tile, Q loads per row tile.
     if (warp < kTcTiles * 4) {
         // =============================== softmax / correction / epilogue ===============================
         const int t = warp >> 2;
@@ -1390,7 +1388,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             bool ok = true;
             long long ring_n = 0;                   // ring items requested so far (K_0, V_0, K_1, ... of every item)
             int q_loads[kTcTiles] = {0, 0};
-            int tails = 0;
+            int tails = 0;                          // tiles cleaned up so far
+            bool tail_pending = false;
             // fused append: tiles waiting to be stored into the cache, per ring slot
             bool store_pending[kTcStages] = {};
             long long store_ring[kTcStages] = {};
@@ -1484,43 +1483,30 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                                 row0 = (kExt & kExtBias) ? (it.j0 + it.nsteps - 1 - (item >> 1)) * kTcKeys : row0 - it.np * kTcKeys;
                             }
                         }
-                        mbar_arrive_expect_tx(bar_kv_full(slot), kTcTileBytes);
+                        // The V tile with rows past the sequence's end (the last one, the first where the keys are walked
+                        // backwards) lands on a barrier of the producer's own; it is cleaned up and only then signalled.
+                        const bool tail = it.zero_tail && item == ((kExt & kExtBias) ? 1 : 2 * it.nsteps - 1);
+                        const uint32_t landed = tail ? bar_tail : bar_kv_full(slot);
+                        mbar_arrive_expect_tx(landed, kTcTileBytes);
                         for (int h = 0; h < 2; ++h)
-                            tma_load_4d(smem_base + kTcSmemRing + slot * kTcTileBytes + h * kTcHalfBytes, map, bar_kv_full(slot),
-                                        h * 64, row0, it.kvh, seq);
-                        if constexpr ((kExt & kExtBias) != 0)
-                            if (it.zero_tail && item == 1) {   // walked backwards: the tile to clean up is the first V tile
-                                ok = mbar_wait(bar_kv_full(slot), round_par, abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
-                                if (!ok) break;
-                                const int first = static_cast<int>(it.key_end - static_cast<long long>(row0));
-                                unsigned char* tile = smem + kTcSmemRing + slot * kTcTileBytes;
-                                for (int r = first * 8; r < kTcKeys * 8; ++r) {
-                                    *reinterpret_cast<uint4*>(tile + r * 16) = make_uint4(0u, 0u, 0u, 0u);
-                                    *reinterpret_cast<uint4*>(tile + kTcHalfBytes + r * 16) = make_uint4(0u, 0u, 0u, 0u);
-                                }
-                                fence_async_smem();
-                                mbar_arrive(bar_tail);
+                            tma_load_4d(smem_base + kTcSmemRing + slot * kTcTileBytes + h * kTcHalfBytes, map, landed, h * 64, row0, it.kvh, seq);
+                        if (tail) {
+                            ok = mbar_wait(bar_tail, static_cast<uint32_t>(tails & 1), abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
+                            if (!ok) {
+                                tail_pending = true;
+                                break;
                             }
-                    }
-                }
-                if ((kExt & kExtBias) == 0 && ok && it.zero_tail && it.nsteps > 0) {
-                    const long long last = ring_n - 1;   // the last V tile
-                    const int slot = static_cast<int>(last % kTcStages);
-                    ok = mbar_wait(bar_kv_full(slot), static_cast<uint32_t>((last / kTcStages) & 1), abort_word, p.status, kTcWaitKvFull,
-                                   p.wait_timeout_ns);
-                    if (ok) {
-                        // a 128-byte row of either half holds one key; the swizzle only permutes inside a row
-                        const int first = static_cast<int>(it.key_end - static_cast<long long>(it.j0 + it.nsteps - tc_prefix_tiles(it) - 1) * kTcKeys);
-                        unsigned char* tile = smem + kTcSmemRing + slot * kTcTileBytes;
-                        for (int r = first; r < kTcKeys; ++r)
-                            for (int h = 0; h < 2; ++h) {
-                                uint4* rowp = reinterpret_cast<uint4*>(tile + h * kTcHalfBytes + r * 128);
-#pragma unroll
-                                for (int c = 0; c < 8; ++c) rowp[c] = make_uint4(0u, 0u, 0u, 0u);
+                            // a 128-byte row of either half holds one key; the swizzle only permutes inside a row
+                            const int first = static_cast<int>(it.key_end - static_cast<long long>(row0));
+                            unsigned char* tile = smem + kTcSmemRing + slot * kTcTileBytes;
+                            for (int r = first * 8; r < kTcKeys * 8; ++r) {
+                                *reinterpret_cast<uint4*>(tile + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                *reinterpret_cast<uint4*>(tile + kTcHalfBytes + r * 16) = make_uint4(0u, 0u, 0u, 0u);
                             }
-                        fence_async_smem();
-                        mbar_arrive(bar_tail);
-                        ++tails;
+                            fence_async_smem();
+                            mbar_arrive(bar_kv_full(slot));
+                            ++tails;
+                        }
                     }
                 }
             }
@@ -1539,8 +1525,8 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 for (int t = 0; t < kTcTiles; ++t)
                     if (q_loads[t] > 0) mbar_wait_quiet(bar_q(t), static_cast<uint32_t>((q_loads[t] - 1) & 1), 200000ull);
+                if (tail_pending) mbar_wait_quiet(bar_tail, static_cast<uint32_t>(tails & 1), 200000ull);
             }
-            (void)tails;
         }
         __syncwarp();
     } else if (kSplit && warp >= kTcTiles * 4 + 2) {
@@ -1633,7 +1619,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     ring_par ^= 1;
                 }
             };
-            unsigned steps_done[kTcTiles] = {0, 0}, q_loads[kTcTiles] = {0, 0}, tails = 0;
+            unsigned steps_done[kTcTiles] = {0, 0}, q_loads[kTcTiles] = {0, 0};
             Item it;
             for (long long k = 0; ok; ++k) {
                 int idx = n_items;
@@ -1645,9 +1631,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (idx >= n_items) break;
                 tc_item(p, idx, it);
                 const int nsteps = it.nsteps;
-                auto wait_tile = [&](int item) -> bool {   // ring item `item` of this work item sits in ring_slot
-                    if (it.zero_tail && item == ((kExt & kExtBias) ? 1 : 2 * nsteps - 1))   // released by the producer's clean-up
-                        return wait(bar_tail, tails & 1u, kTcWaitKvFull);
+                auto wait_tile = [&]() -> bool {   // the next tile of the ring
                     return wait(bar_kv_full(ring_slot), ring_par, kTcWaitKvFull);
                 };
                 auto issue_qk = [&](int t, int slot, bool last) {
@@ -1677,7 +1661,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int t = 0; t < kTcTiles && ok; ++t)
                     if (it.steps[t] > 0) ok = wait(bar_q(t), q_loads[t] & 1u, kTcWaitQ);
                 if (ok && nsteps > 0) {
-                    ok = wait_tile(0);
+                    ok = wait_tile();
                     if (ok) {
                         tc_fence_after();
                         for (int t = 0; t < kTcTiles; ++t)
@@ -1694,7 +1678,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         ok = wait(bar_p_full(t), (steps_done[t] + j) & 1u, kTcWaitPFull);
                         if (!ok) break;
                         if (!have_v) {
-                            ok = wait_tile(2 * j + 1);
+                            ok = wait_tile();
                             if (!ok) break;
                             slot_v = ring_slot;
                             next_slot();
@@ -1704,7 +1688,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         issue_pv(t, slot_v, j == 0);
                         if (j + 1 < it.steps[t]) {
                             if (!have_k) {
-                                ok = wait_tile(2 * j + 2);
+                                ok = wait_tile();
                                 if (!ok) break;
                                 slot_k = ring_slot;
                                 next_slot();
@@ -1722,7 +1706,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     __syncwarp();
                 }
                 if (!ok) break;
-                if (it.zero_tail && nsteps > 0) ++tails;
                 for (int t = 0; t < kTcTiles; ++t) {
                     steps_done[t] += it.steps[t];
                     if (it.steps[t] > 0) ++q_loads[t];
@@ -1767,7 +1750,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             long long ring_c = 0;                  // ring items of all earlier work items
             int steps_done[kTcTiles] = {0, 0};
             int q_loads[kTcTiles] = {0, 0};
-            int tails = 0;
             Item it;
             for (long long k = 0; ok; ++k) {
                 const int idx = take_item(k, ok, kTcWaitSched);
@@ -1779,8 +1761,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // ring item i of this work item: K_(i/2) for even i, V_(i/2) for odd i
                 auto wait_item = [&](int item) {
                     const long long r = ring_c + item;
-                    if (it.zero_tail && item == 2 * nsteps - 1)   // the last V tile is released by the producer's clean-up
-                        return mbar_wait(bar_tail, static_cast<uint32_t>(tails & 1), abort_word, p.status, kTcWaitKvFull, p.wait_timeout_ns);
                     return mbar_wait(bar_kv_full(static_cast<int>(r % kTcStages)), static_cast<uint32_t>((r / kTcStages) & 1), abort_word,
                                      p.status, kTcWaitKvFull, p.wait_timeout_ns);
                 };
@@ -1833,7 +1813,6 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 if (!ok) break;
                 ring_c += 2 * nsteps;
-                if (it.zero_tail && nsteps > 0) ++tails;
                 for (int t = 0; t < kTcTiles; ++t) {
                     steps_done[t] += it.steps[t];
                     if (it.steps[t] > 0) ++q_loads[t];
