@@ -799,7 +799,7 @@ __device__ __forceinline__ float tc_first_max(uint32_t tS, const TcRow& r, int l
 // a score leaps far above the maximum in use.  32 columns at a time in a rolled
 // loop: it is rare, and its code must not push the one-pass step's out of the instruction cache.
 template <int kExt>
-__device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRow& r, int lo, int rel, bool rescale_o, float& m_used, float& l) {
+__device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRow& r, int lo, int rel, bool rescale_o, bool valid, float& m_used, float& l) {
     float mx = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
@@ -814,7 +814,7 @@ __device__ __forceinline__ void tc_two_pass(uint32_t tS, uint32_t tO, const TcRo
     }
     const float m_new = fmaxf(m_used, mx);
     const bool need = (m_new - m_used > kTcRescaleThreshold) || (m_used == -INFINITY && m_new != -INFINITY);
-    const bool rescale = __any_sync(0xffffffffu, need);
+    const bool rescale = __any_sync(0xffffffffu, need && valid);   // (lanes without a row hold left-overs)
     float corr = 1.0f;
     if (rescale) {
         corr = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
@@ -889,7 +889,7 @@ __device__ __forceinline__ void tc_step_ext(uint32_t tS, uint32_t tO, const TcRo
             }
         }
     }
-    if (slow) tc_two_pass<kExt>(tS, tO, r, edge ? lo : 0, edge ? rel : 127, !first, m_used, l);
+    if (slow) tc_two_pass<kExt>(tS, tO, r, edge ? lo : 0, edge ? rel : 127, !first, valid, m_used, l);
 }
 
 // kFused: the chunk's own K/V rows come from k_new / v_new and are written into the cache here (a
