@@ -628,13 +628,19 @@ __device__ __noinline__ TcFixed tc_fix_second_half(uint32_t tS, uint32_t tO, flo
         }
         mx = max3(mx, max3(m0, v[30], v[31]), m1);
     }
-    const float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * scale_log2);
+    float m_new = fmaxf(m_used, kExt != 0 ? mx : mx * scale_log2);
     // rows whose maximum did not move far keep it (their corr is 1): as in the two-pass step
     bool moved = m_new - m_used > kTcRescaleThreshold;
     if constexpr (kExt != 0) moved = moved && m_new != -INFINITY;
     float corr = moved ? fast_exp2(m_used - m_new) : 1.0f;
-    if constexpr (kExt != 0)   // a row whose first key is in this half: nothing to bring along
-        if (moved && m_used == -INFINITY) corr = 0.0f;
+    if constexpr (kExt != 0)
+        if (moved) {
+            // The row moves by whole powers of two (to less than 1 above its maximum), so that the first half's P, rounded to
+            // bf16 already, is not rounded again.  A row whose first key is in this half has nothing to bring along.
+            const float by = ceilf(m_new - m_used);
+            corr = by < 126.0f ? __int_as_float((127 - static_cast<int>(by)) << 23) : 0.0f;
+            if (m_used != -INFINITY) m_new = m_used + by;
+        }
     if (moved) m_used = m_new;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {   // O_t: every P.V of earlier steps has completed (this step's S_t exists)
