@@ -750,24 +750,19 @@ __device__ __forceinline__ float tc_row64(float (&s)[64], const TcRow& r, const 
     const float d = r.dist0 - c0, base = (kExt & kExtBias) ? off - r.slope * d : off;
     bool direct = true;
     if constexpr ((kExt & kExtCap) != 0) {
-        // Which form the warp takes follows from what its rows see alone: lanes without a row, whose queries are whatever the
-        // tile held before, have no say, and masked products only appear to (they are taken out before the warp gives up).
-        auto in_range = [&]() -> bool {
-            float a0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), a1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
-#pragma unroll
-            for (int i = 6; i < 62; i += 4) {
-                a0 = max3(a0, fabsf(s[i]), fabsf(s[i + 1]));
-                a1 = max3(a1, fabsf(s[i + 2]), fabsf(s[i + 3]));
-            }
-            a0 = max3(a0, fabsf(s[62]), fabsf(s[63]));
-            return __all_sync(0xffffffffu, fmaxf(a0, a1) * r.cap_in <= kTanhPolyMax || !valid);
-        };
-        direct = in_range();
-        if (!direct && edge) {
+        // Which form the warp takes follows from what its rows see alone: masked products count as 0, and lanes without a
+        // row, whose queries are whatever the tile held before, have no say.
+        if (edge)
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u ? s[i] : 0.0f;
-            direct = in_range();
+        float a0 = max3(fabsf(s[0]), fabsf(s[1]), fabsf(s[2])), a1 = max3(fabsf(s[3]), fabsf(s[4]), fabsf(s[5]));
+#pragma unroll
+        for (int i = 6; i < 62; i += 4) {
+            a0 = max3(a0, fabsf(s[i]), fabsf(s[i + 1]));
+            a1 = max3(a1, fabsf(s[i + 2]), fabsf(s[i + 3]));
         }
+        a0 = max3(a0, fabsf(s[62]), fabsf(s[63]));
+        direct = __all_sync(0xffffffffu, fmaxf(a0, a1) * r.cap_in <= kTanhPolyMax || !valid);
     }
     if constexpr ((kExt & kExtBias) != 0) direct = direct && r.ahead;
     if (direct) return edge ? tc_exp64<kExt, false, true>(s, r, coef, base, m0, m1, pk) : tc_exp64<kExt, false, false>(s, r, coef, base, m0, m1, pk);
