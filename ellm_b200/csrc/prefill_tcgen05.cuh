@@ -37,9 +37,9 @@
 // What bounds it: the softmax warps.  A 128-key step of both row tiles takes about 3700 clocks plain, 5000 capped
 // (six multiply-adds a score for the tanh) and 4300 biased, against 2800 for its products; an item costs about
 // 11000 clocks besides its steps (queries, first tile, epilogue), which is what short documents and windows pay.
-// Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.6 to 2.75 ms by the GPU's clocks (800 to 850
-// TFLOP/s); 2 x 8191 tokens of documents of about 900, biased, 32 / 8 heads, 373 us; 8 x 256 rows under a capped 1024-key
-// window, 64 / 8 heads, 141 us; 16 x 48 rows after 8190 shared keys, 32 / 4 heads, 162 us (640 TFLOP/s).
+// Measured, 128-element heads: capped 16384-token prompt, 32 / 4 heads, 2.55 to 2.75 ms by the GPU's clocks (800 to 860
+// TFLOP/s); 2 x 8191 tokens of documents of about 900, biased, 32 / 8 heads, 374 us; 8 x 256 rows under a capped 1024-key
+// window, 64 / 8 heads, 145 us; 16 x 48 rows after 8190 shared keys, 32 / 4 heads, 159 us (650 TFLOP/s).
 // An item owns all keys of its rows: a chunk of fewer items than SMs leaves the others idle (1 x 64 rows after 8190 keys is
 // 8 items, 188 us capped; 1 x 16 rows after 32768 shared keys 4 items, 507 us).
 //
