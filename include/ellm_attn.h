@@ -112,7 +112,7 @@ int ellm_attn_run_ragged(ellm_attn* h, const int32_t* positions, size_t position
  * runs, copies out (and lse) back, and returns when the results are in host
  * memory.  The KV cache stays resident on the device.  Decode steps with positions_host and
  * page-locked buffers are captured once into a CUDA graph and replayed for as long as the same
- * buffers are passed; in that graph one small kernel fetches all inputs from the host buffers
+ * buffers are passed and no option, scores or shared prefix are set in between; in that graph one small kernel fetches all inputs from the host buffers
  * and the last kernel of the step stores O and LSE directly into out_host / lse_host, so the
  * handle's device out / lse buffers are not written by such a step.  Calls on one handle must
  * not overlap. */
@@ -269,6 +269,7 @@ int ellm_step_graph_destroy(ellm_step_graph* graph);
  *                included; they have to lie in one chunk (a row cannot see keys not yet written).
  * Two things are right but slow: chunks with softcap > 128 (or scale / softcap outside [1/4096, 2048]) run
  * on the warp-level kernel, and rows whose 128-key tiles hold NaN or infinity are computed once more, key by key.
+ * Scores are fp32: one of some thousands (a steep negative slope over a long distance) is known to 2^-24 of itself.
  * All arrays are device memory, read by every run; they have to stay valid and may be rewritten between
  * runs.  The distance is that of positions in the handle's cache.  The struct is copied; s NULL, or one
  * without any part set, goes back to plain attention.  Not together with ellm_attn_set_shared_prefix
